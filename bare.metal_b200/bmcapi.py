@@ -44,6 +44,12 @@ class Backend:
         lib.bmc_cast_f32_to_bf16.argtypes = [vp, vp, vp, sz]
         lib.bmc_cast_bf16_to_f32.argtypes = [vp, vp, vp, sz]
         lib.bmc_seq_prefix_accumulate.argtypes = [vp, ci, vp, vp, ci, sz]
+        lib.bmc_stream.restype = vp
+        lib.bmc_stream.argtypes = [vp]
+        lib.bmc_quantize_rows_q8.argtypes = [vp, ci, vp, ci, vp, vp, ci, ci, ci]
+        lib.bmc_rmsnorm_q8.argtypes = [vp, ci, vp, ci, vp, vp, ci, vp, ci, ci, vp, ci, vp, ci, ci, cf]
+        lib.bmc_swiglu_q8.argtypes = [vp, ci, vp, ci, vp, vp, vp, ci, ci, ci]
+        lib.bmc_matmul_q8.argtypes = [vp, ci, vp, ci, vp, ci, vp, vp, vp, vp, ci, ci, ci, ci]
         self.ctx = lib.bmc_create(0)
         if not self.ctx:
             raise RuntimeError("bmc_create(0) failed: no sm_100 GPU (the backend has no CPU fallback)")

@@ -15,6 +15,7 @@
 #include "decode_kernels.cuh"
 #include "gemm_umma.cuh"
 #include "kernels.cuh"
+#include "q8_kernels.cuh"
 
 using namespace bmb;
 namespace bmb { int wait_probe_launch(int* err, cudaStream_t st); }
@@ -103,6 +104,25 @@ int run_umma(bmc_ctx_t* ctx, const GemmProblem& g) {
     ctx->gt_flops[ctx->gt_used] = 2.0 * g.M * g.N * g.K;
     ctx->gt_used++;
     return rc;
+}
+
+// The context's device is current for the duration of a call, whatever device the calling thread had selected.
+struct DeviceScope {
+    int before = -1, mine;
+    explicit DeviceScope(int device) : mine(device) {
+        if (cudaGetDevice(&before) == cudaSuccess && before != mine) cudaSetDevice(mine);
+    }
+    ~DeviceScope() {
+        if (before >= 0 && before != mine) cudaSetDevice(before);
+    }
+};
+
+bool is_dtype(int dtype) { return dtype == BMC_F32 || dtype == BMC_BF16; }
+bool misaligned(const void* p, int dtype) { return ((uintptr_t)p & (dtype == BMC_F32 ? 3u : 1u)) != 0; }
+// what the three row operators have in common: 0 = go on
+int check_q8_rows(int dtype, const void* q, int ldq, const void* scale, const void* x, int ldx, int rows, int C) {
+    if (!is_dtype(dtype) || rows < 0 || C < 1 || C > BMC_Q8_MAX_COLUMNS || ldq < C || ldx < C || !q || !scale || !x) return -1;
+    return misaligned(scale, BMC_F32) || misaligned(x, dtype) ? -3 : 0;
 }
 
 }  // namespace
@@ -668,6 +688,49 @@ int bmc_decode_argmax_advance(bmc_ctx_t* ctx, int* d_out, const float* d_logits,
 int bmc_decode_advance(bmc_ctx_t* ctx, int* d_pos) {
     BMC_CHECK_CTX(ctx);
     return note(ctx, decode_advance(d_pos, ctx->stream));
+}
+
+// ---- 8-bit rows and their product --------------------------------------------------------------------
+static_assert(BMC_Q8_MAX_COLUMNS == Q8_MAX_COLUMNS, "header and kernels agree");
+int bmc_quantize_rows_q8(bmc_ctx_t* ctx, int dtype, int8_t* d_q, int ldq, float* d_scale, const void* d_x, int ldx, int rows, int C) {
+    BMC_CHECK_CTX(ctx);
+    if (const int rc = check_q8_rows(dtype, d_q, ldq, d_scale, d_x, ldx, rows, C)) return rc;
+    if (rows == 0) return 0;
+    DeviceScope on(ctx->device);
+    return note(ctx, q8_quantize_rows(dtype, d_q, ldq, d_scale, d_x, ldx, rows, C, ctx->stream));
+}
+int bmc_rmsnorm_q8(bmc_ctx_t* ctx, int dtype, int8_t* d_q, int ldq, float* d_scale, void* d_sum, int lds, const void* d_x, int ldx, int add_dtype,
+                   const void* d_add, int lda, const float* d_w, int rows, int C, float eps) {
+    BMC_CHECK_CTX(ctx);
+    if (const int rc = check_q8_rows(dtype, d_q, ldq, d_scale, d_x, ldx, rows, C)) return rc;
+    if (!d_w || (d_add && (!is_dtype(add_dtype) || lda < C)) || (d_sum && lds < C)) return -1;
+    if (d_sum && ((d_sum == d_x && lds != ldx) || (d_sum == d_add && (lds != lda || add_dtype != dtype)))) return -1;
+    if (misaligned(d_w, BMC_F32) || (d_add && misaligned(d_add, add_dtype)) || (d_sum && misaligned(d_sum, dtype))) return -3;
+    if (rows == 0) return 0;
+    DeviceScope on(ctx->device);
+    return note(ctx, q8_rmsnorm(dtype, d_q, ldq, d_scale, d_sum, lds, d_x, ldx, add_dtype, d_add, lda, d_w, rows, C, eps, ctx->stream));
+}
+int bmc_swiglu_q8(bmc_ctx_t* ctx, int dtype, int8_t* d_q, int ldq, float* d_scale, const void* d_gate, const void* d_up, int ldgu, int rows, int H) {
+    BMC_CHECK_CTX(ctx);
+    if (const int rc = check_q8_rows(dtype, d_q, ldq, d_scale, d_gate, ldgu, rows, H)) return rc;
+    if (!d_up) return -1;
+    if (misaligned(d_up, dtype)) return -3;
+    if (rows == 0) return 0;
+    DeviceScope on(ctx->device);
+    return note(ctx, q8_swiglu(dtype, d_q, ldq, d_scale, d_gate, d_up, ldgu, rows, H, ctx->stream));
+}
+int bmc_matmul_q8(bmc_ctx_t* ctx, int dtype, void* d_out, int ldo, const int8_t* d_q, int ldq, const float* d_scale, const int8_t* d_w,
+                  const float* d_w_scale, const void* d_residual, int ldr, int BT, int C, int OC) {
+    BMC_CHECK_CTX(ctx);
+    if (!is_dtype(dtype) || BT < 0 || OC < 0 || C < 1 || C > BMC_Q8_MAX_K || ldq < C || ldo < OC || (d_residual && ldr < OC)) return -1;
+    if (!d_out || !d_q || !d_scale || !d_w || !d_w_scale || (d_residual == d_out && ldr != ldo)) return -1;
+    if ((C % 16) || (ldq % 16)) return -2;
+    if ((((uintptr_t)d_q | (uintptr_t)d_w) & 15) || misaligned(d_scale, BMC_F32) || misaligned(d_w_scale, BMC_F32) || misaligned(d_out, dtype) ||
+        (d_residual && misaligned(d_residual, dtype)))
+        return -3;
+    if (BT == 0 || OC == 0) return 0;
+    DeviceScope on(ctx->device);
+    return note(ctx, q8_matmul(dtype, d_out, ldo, d_q, ldq, d_scale, d_w, d_w_scale, d_residual, ldr, BT, C, OC, ctx->d_err, ctx->stream));
 }
 int bmc_graph_select(bmc_ctx_t* ctx, int slot) {
     BMC_CHECK_CTX(ctx);

@@ -1,0 +1,21 @@
+// Launchers of the 8-bit activation operators (q8_rows.cu, q8_matmul.cu). dtype 0 = fp32, 1 = bf16 (BMC_F32 / BMC_BF16).
+// Arguments are checked by the entry points (backend_api.cu); every launcher enqueues on `st` and returns 0 or a negative code.
+#pragma once
+#include "common.cuh"
+
+namespace bmb {
+
+// widest row of the row kernels: one fp32 value per column in shared memory
+constexpr int Q8_MAX_COLUMNS = 57344;
+
+int q8_quantize_rows(int dtype, int8_t* q, int ldq, float* scale, const void* x, int ldx, int rows, int C, cudaStream_t st);
+// add, sum and their combination are optional (null); sum may be x or add
+int q8_rmsnorm(int dtype, int8_t* q, int ldq, float* scale, void* sum, int lds, const void* x, int ldx, int add_dtype, const void* add, int lda,
+               const float* w, int rows, int C, float eps, cudaStream_t st);
+int q8_swiglu(int dtype, int8_t* q, int ldq, float* scale, const void* gate, const void* up, int ldgu, int rows, int H, cudaStream_t st);
+
+// out[m, n] = (sum_k q[m, k] w[n, k]) * (scale[m] * wscale[n]) (+ residual[m, n])
+int q8_matmul(int dtype, void* out, int ldo, const int8_t* q, int ldq, const float* scale, const int8_t* w, const float* wscale, const void* residual,
+              int ldr, int M, int K, int N, int* err, cudaStream_t st);
+
+}  // namespace bmb

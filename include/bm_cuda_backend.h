@@ -252,6 +252,35 @@ int bmc_graph_begin(bmc_ctx_t* ctx);
 int bmc_graph_end(bmc_ctx_t* ctx);
 int bmc_graph_launch(bmc_ctx_t* ctx);
 
+/* ---- 8-bit rows and their product (activations in 8 bits; no counterpart in the reference, whose Q8 / Q4 keep fp32 activations) ----
+ * A matrix in 8 bits is int8 codes [rows][ld] and one fp32 scale per row; it stands for code * scale. Activations have a scale per token,
+ * weights ([OC][C], rows = output channels) a scale per channel: bmc_quantize_rows_q8 makes both.
+ *   row v[C]:  scale = max|v| / 127, code = rint(v * (1 / scale)), ties to even; codes lie in [-127, 127].
+ *   A row whose scale would be subnormal (max|v| < 1.5e-36, zeros) is stored as scale 0 and codes 0. A row with an infinity or a NaN, in v
+ *   or on the way to it (a sum of squares that overflows), is stored as scale NaN and codes 0: its products are NaN.
+ * dtype / add_dtype: BMC_F32 or BMC_BF16, arithmetic in fp32. Every leading dimension is in elements and at least the row's width; columns
+ * behind C are neither read nor written. Rows of any width 1 <= C <= BMC_Q8_MAX_COLUMNS and any alignment of their type; 16-byte aligned
+ * pointers and leading dimensions take the vectorised path. Zero rows: 0 is returned and nothing is enqueued. Outputs may not overlap
+ * inputs, except where said. Return values: 0, -1 (an argument out of range or a null pointer), -2 (a leading dimension that is no
+ * multiple of what the call asks for), -3 (a misaligned pointer). Nothing is enqueued by a refused call.
+ *   quantize_rows : v = x
+ *   rmsnorm       : v = s * rsqrt(mean(s^2) + eps) * w with s = x + add (add may be NULL: s = x); the norm takes s before it is rounded.
+ *                   d_sum (may be NULL) receives s in dtype; it may be d_x itself (lds == ldx), or d_add (same dtype, lds == lda).
+ *                   Follows rmsnorm_forward_v2 (forward.metal:1019) behind add_forward (forward.metal:1332).
+ *   swiglu        : v = silu(gate) * up (swiglu_forward, forward.metal:1179); gate and up share the leading dimension, as [gate | up] rows do.
+ *   matmul        : out[BT,OC] = (sum_c q[BT,c] * w[OC,c]) * (scale[BT] * w_scale[OC]) (+ residual[BT,OC] in dtype; it may be d_out itself,
+ *                   ldr == ldo). The sum is an exact 32-bit integer, so results do not depend on its order. 1 <= C <= BMC_Q8_MAX_K; C and ldq
+ *                   are multiples of 16 and d_q, d_w 16-byte aligned (pad rows with zero codes); codes may be -128. d_w is [OC][C] without
+ *                   gaps. BT and OC are arbitrary (0: nothing is enqueued). ---- */
+#define BMC_Q8_MAX_COLUMNS 57344
+#define BMC_Q8_MAX_K 131056
+int bmc_quantize_rows_q8(bmc_ctx_t* ctx, int dtype, int8_t* d_q, int ldq, float* d_scale, const void* d_x, int ldx, int rows, int C);
+int bmc_rmsnorm_q8(bmc_ctx_t* ctx, int dtype, int8_t* d_q, int ldq, float* d_scale, void* d_sum, int lds, const void* d_x, int ldx, int add_dtype,
+                   const void* d_add, int lda, const float* d_w, int rows, int C, float eps);
+int bmc_swiglu_q8(bmc_ctx_t* ctx, int dtype, int8_t* d_q, int ldq, float* d_scale, const void* d_gate, const void* d_up, int ldgu, int rows, int H);
+int bmc_matmul_q8(bmc_ctx_t* ctx, int dtype, void* d_out, int ldo, const int8_t* d_q, int ldq, const float* d_scale, const int8_t* d_w,
+                  const float* d_w_scale, const void* d_residual, int ldr, int BT, int C, int OC);
+
 #ifdef __cplusplus
 }
 #endif
