@@ -4,9 +4,14 @@
 // The maximum is taken over the bit patterns of |v| as unsigned integers: they order like the values, and an infinity or NaN is larger than
 // every number, so one reduction also says whether the row can be stored. A row that holds such a value gets the scale NaN (and codes 0),
 // which every product with it carries on; a row whose scale would be subnormal (max|v| < 1.5e-36, a row of zeros among them) gets scale 0.
-// No clamp is needed: scale, 1 / scale and the product are each rounded once from normal numbers, so |v| / scale stays below
-// 127 * (1 + 2^-22) and rounds to 127 at most.
+// No clamp is needed: scale and 1 / scale are each rounded once from normal numbers, so |v| / scale stays below 127 * (1 + 2^-22) and
+// rounds to 127 at most.
+//
+// All three are bound by memory: every input is read once and every output written once, the row stays in registers between the reductions
+// (up to 32 values a thread), so the threads of a row follow from its width.
 #include "q8_kernels.cuh"
+
+#include <cstdlib>
 
 namespace bmb {
 
@@ -20,51 +25,198 @@ struct RowArgs {
     const void *x, *y;   // y: the addend (norm), the up projection (SwiGLU)
     void* sum;
     const float* w;
-    int ldq, ldx, ldy, lds, C;
+    int ldq, ldx, ldy, lds, C, rows;
     float eps;
 };
 
-__device__ __forceinline__ float silu(float g) { return g / (1.0f + expf(-g)); }
+constexpr uint32_t INF_BITS = 0x7f800000u;
+__device__ __forceinline__ float quiet_nan() { return __uint_as_float(0x7fc00000u); }
+__device__ __forceinline__ uint32_t abs_bits(float f) { return __float_as_uint(f) & 0x7fffffffu; }
 
-__device__ __forceinline__ float block_sum(float v, float* red) {
-    v = warp_sum(v);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float t = 0.0f;
-    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) t += red[i];
-    __syncthreads();
-    return t;
-}
-__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
-    v = __reduce_max_sync(0xffffffffu, v);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    uint32_t t = 0;
-    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) t = max(t, red[i]);
-    return t;
-}
+// g / (1 + exp(-g)): the exponential is one special-function instruction on -g * log2(e) (relative error 2^-22 + 2 |g| 2^-24), the quotient
+// a reciprocal and a product (2 units in the last place). For g < -88 the exponential is infinite and the quotient -0.
+__device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.0f + __expf(-g)); }
 
-// scale and 1 / scale of a row whose largest |v| has the bit pattern `top`
+// scale and 1 / scale of a row whose largest |v| has the bit pattern `top`; inv = 0 where every code is 0
 __device__ __forceinline__ float row_scale(uint32_t top, float& inv) {
-    if (top >= 0x7f800000u) {
-        inv = 0.0f;
-        return __uint_as_float(0x7fc00000u);
-    }
+    inv = 0.0f;
+    if (top >= INF_BITS) return quiet_nan();
     const float s = __uint_as_float(top) / 127.0f;
-    if (s < 1.17549435e-38f) {
-        inv = 0.0f;
-        return 0.0f;
-    }
+    if (s < 1.17549435e-38f) return 0.0f;
     inv = 1.0f / s;
     return s;
 }
+// 1 / rms of a row. A sum of squares that overflowed has no reciprocal root: the row becomes NaN, not zero.
+__device__ __forceinline__ float row_rstd(float ss, int C, float eps) {
+    return ss < __uint_as_float(INF_BITS) ? 1.0f / sqrtf(ss / (float)C + eps) : quiet_nan();
+}
+// the code of v in the low byte: adding 1.5 * 2^23 leaves rint(v * inv) in the mantissa's low bits, in two's complement, without the
+// conversion unit (a quarter of the rate). A NaN, which only a row with inv = 0 holds, is replaced before.
+__device__ __forceinline__ uint32_t code_bits(float v, float inv) { return __float_as_uint(__fmaf_rn(v, inv, 12582912.0f)); }
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
 
-// One block per row, the row's values in shared memory between the passes.
+// N consecutive elements as floats, in the widest loads their size allows
+template <typename T, int N> struct Pack;
+template <typename T> struct Pack<T, 1> {
+    T v;
+    __device__ __forceinline__ void load(const T* p) { v = *p; }
+    __device__ __forceinline__ void unpack(float (&f)[1]) const { f[0] = to_f32(v); }
+    __device__ __forceinline__ static void store(T* p, const float (&f)[1]) { *p = from_f32<T>(f[0]); }
+};
+template <> struct Pack<float, 4> {
+    float4 v;
+    __device__ __forceinline__ void load(const float* p) { v = *(const float4*)p; }
+    __device__ __forceinline__ void unpack(float (&f)[4]) const { f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
+    __device__ __forceinline__ static void store(float* p, const float (&f)[4]) { Vec<float>::store(p, f); }
+};
+template <> struct Pack<float, 8> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p) { a = *(const float4*)p; b = *(const float4*)(p + 4); }
+    __device__ __forceinline__ void unpack(float (&f)[8]) const { f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w; }
+};
+template <> struct Pack<bf16, 4> {
+    uint2 v;
+    __device__ __forceinline__ void load(const bf16* p) { v = *(const uint2*)p; }
+    __device__ __forceinline__ void unpack(float (&f)[4]) const {
+        f[0] = __uint_as_float(v.x << 16); f[1] = __uint_as_float(v.x & 0xffff0000u);
+        f[2] = __uint_as_float(v.y << 16); f[3] = __uint_as_float(v.y & 0xffff0000u);
+    }
+};
+template <> struct Pack<bf16, 8> {
+    uint4 v;
+    __device__ __forceinline__ void load(const bf16* p) { v = Vec<bf16>::load_raw(p); }
+    __device__ __forceinline__ void unpack(float (&f)[8]) const { Vec<bf16>::unpack(v, f); }
+    __device__ __forceinline__ static void store(bf16* p, const float (&f)[8]) { Vec<bf16>::store(p, f); }
+};
+
+template <int N> __device__ __forceinline__ void store_codes(int8_t* p, const float (&f)[N], float inv) {
+    if constexpr (N == 1) {
+        *p = (int8_t)code_bits(f[0], inv);
+    } else {
+        uint32_t w[N / 4];
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) w[i] = pack4(code_bits(f[4 * i], inv), code_bits(f[4 * i + 1], inv), code_bits(f[4 * i + 2], inv), code_bits(f[4 * i + 3], inv));
+        if constexpr (N == 4) *(uint32_t*)p = w[0];
+        else *(uint2*)p = make_uint2(w[0], w[1]);
+    }
+}
+
+// Reductions over the threads of a row: one warp (WARP), or the block.
+template <bool WARP> __device__ __forceinline__ float row_sum(float v, float* red) {
+    v = warp_sum(v);
+    if (WARP) return v;
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    const int n = blockDim.x >> 5;
+    return warp_sum((int)(threadIdx.x & 31) < n ? red[threadIdx.x & 31] : 0.0f);
+}
+template <bool WARP> __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* red) {
+    v = __reduce_max_sync(0xffffffffu, v);
+    if (WARP) return v;
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    const int n = blockDim.x >> 5;
+    return __reduce_max_sync(0xffffffffu, (int)(threadIdx.x & 31) < n ? red[threadIdx.x & 31] : 0u);
+}
+
+constexpr int WARP_ROWS = 4;   // rows per block where a warp has a row
+
+// V elements per access, NV accesses per thread. WARP: a warp per row, WARP_ROWS rows per block; otherwise a block per row.
+template <int MODE, typename TX, typename TY, int V, int NV, bool WARP>
+__global__ void __launch_bounds__(WARP ? 32 * WARP_ROWS : 512) q8_row_kernel(const RowArgs p) {
+    __shared__ float red[32];
+    __shared__ uint32_t redu[32];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int row = WARP ? (int)blockIdx.x * WARP_ROWS + (int)(threadIdx.x >> 5) : (int)blockIdx.x;
+    const int t = WARP ? (int)(threadIdx.x & 31) : (int)threadIdx.x, nt = WARP ? 32 : (int)blockDim.x;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (row >= p.rows) return;   // whole warps only, and only where a warp has a row
+    const TX* x = (const TX*)p.x + (size_t)row * p.ldx;
+    const TY* y = (const TY*)p.y + (size_t)row * p.ldy;
+    const bool has_y = MODE == Q8_SWIGLU || (MODE == Q8_NORM && p.y != nullptr);
+    Pack<TX, V> px[NV];
+    Pack<TY, V> py[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (t + i * nt) * V;
+        if (c < p.C) {
+            px[i].load(x + c);
+            if (has_y) py[i].load(y + c);
+        }
+    }
+    float v[NV][V];
+    float ss = 0.0f;
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (t + i * nt) * V;
+        if (c < p.C) {
+            px[i].unpack(v[i]);
+            if (has_y) {
+                float f[V];
+                py[i].unpack(f);
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[i][j] = MODE == Q8_SWIGLU ? silu(v[i][j]) * f[j] : v[i][j] + f[j];
+            }
+            if (MODE == Q8_NORM && p.sum) Pack<TX, V>::store((TX*)p.sum + (size_t)row * p.lds + c, v[i]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[i][j] = 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            if (MODE == Q8_NORM) ss = fmaf(v[i][j], v[i][j], ss);
+            else top = max(top, abs_bits(v[i][j]));
+        }
+    }
+    if (MODE == Q8_NORM) {
+        Pack<float, V> pw[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (t + i * nt) * V;
+            if (c < p.C) pw[i].load(p.w + c);
+        }
+        const float r = row_rstd(row_sum<WARP>(ss, red), p.C, p.eps);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (t + i * nt) * V;
+            if (c < p.C) {
+                float w[V];
+                pw[i].unpack(w);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    v[i][j] = v[i][j] * r * w[j];
+                    top = max(top, abs_bits(v[i][j]));
+                }
+            }
+        }
+    }
+    float inv;
+    const float s = row_scale(row_max<WARP>(top, redu), inv);
+    if (t == 0) p.scale[row] = s;
+    int8_t* q = p.q + (size_t)row * p.ldq;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (t + i * nt) * V;
+        if (c < p.C) {
+            if (inv == 0.0f)
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[i][j] = 0.0f;
+            store_codes<V>(q + c, v[i], inv);
+        }
+    }
+}
+
+// Rows that 512 threads cannot hold in registers: a block per row, the row in shared memory between the passes.
 template <int MODE, typename TX, typename TY>
-__global__ void __launch_bounds__(256) q8_row_kernel(const RowArgs p) {
+__global__ void __launch_bounds__(1024) q8_wide_row_kernel(const RowArgs p) {
     extern __shared__ float v[];
-    __shared__ float red[8];
-    __shared__ uint32_t redu[8];
+    __shared__ float red[32];
+    __shared__ uint32_t redu[32];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const size_t row = blockIdx.x;
     const TX* x = (const TX*)p.x + row * p.ldx;
     const TY* y = p.y ? (const TY*)p.y + row * p.ldy : nullptr;
@@ -76,56 +228,106 @@ __global__ void __launch_bounds__(256) q8_row_kernel(const RowArgs p) {
         if (MODE == Q8_NORM) {
             if (y) f += to_f32(y[c]);
             if (p.sum) ((TX*)p.sum)[row * p.lds + c] = from_f32<TX>(f);
-            ss += f * f;
+            ss = fmaf(f, f, ss);
         }
         v[c] = f;
-        top = max(top, __float_as_uint(f) & 0x7fffffffu);
+        top = max(top, abs_bits(f));
     }
     if (MODE == Q8_NORM) {
-        ss = block_sum(ss, red);
-        // a sum of squares that overflowed has no reciprocal root: the row becomes NaN, not zero
-        const float r = ss < __uint_as_float(0x7f800000u) ? 1.0f / sqrtf(ss / (float)p.C + p.eps) : __uint_as_float(0x7fc00000u);
+        const float r = row_rstd(row_sum<false>(ss, red), p.C, p.eps);
         top = 0;
         for (int c = threadIdx.x; c < p.C; c += blockDim.x) {
             const float f = v[c] * r * p.w[c];
             v[c] = f;
-            top = max(top, __float_as_uint(f) & 0x7fffffffu);
+            top = max(top, abs_bits(f));
         }
     }
-    top = block_max(top, redu);
     float inv;
-    const float s = row_scale(top, inv);
+    const float s = row_scale(row_max<false>(top, redu), inv);
     if (threadIdx.x == 0) p.scale[row] = s;
     int8_t* q = p.q + row * p.ldq;
-    for (int c = threadIdx.x; c < p.C; c += blockDim.x) q[c] = inv == 0.0f ? 0 : (int8_t)__float2int_rn(v[c] * inv);
+    for (int c = threadIdx.x; c < p.C; c += blockDim.x) q[c] = inv == 0.0f ? 0 : (int8_t)code_bits(v[c], inv);
 }
 
-template <int MODE, typename TX, typename TY>
-int launch(const RowArgs& p, int rows, cudaStream_t st) {
-    static std::atomic<unsigned long long> done{0};
-    if (first_use_on_current_device(done))
-        if (cudaFuncSetAttribute(q8_row_kernel<MODE, TX, TY>, cudaFuncAttributeMaxDynamicSharedMemorySize, Q8_MAX_COLUMNS * 4) != cudaSuccess) return -5;
-    q8_row_kernel<MODE, TX, TY><<<rows, 256, (size_t)p.C * 4, st>>>(p);
-    return cudaGetLastError() == cudaSuccess ? 0 : -9;
+// Every kernel here waits for its predecessor itself (griddepcontrol.wait), so it may be launched while that one still runs.
+template <typename K> int launch(K kernel, unsigned grid, unsigned block, size_t smem, const RowArgs& p, cudaStream_t st) {
+    static const bool overlap = getenv("BM_NO_PDL") == nullptr;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = overlap ? 1 : 0;
+    if (cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess) return 0;
+    cudaGetLastError();   // a launch that failed must not poison the status of later calls
+    return -9;
+}
+
+template <int MODE, typename TX, typename TY, int V, int NV> int launch_rows(const RowArgs& p, int threads, cudaStream_t st) {
+    if (threads == 32)
+        return launch(q8_row_kernel<MODE, TX, TY, V, NV, true>, (unsigned)((p.rows + WARP_ROWS - 1) / WARP_ROWS), 32 * WARP_ROWS, 0, p, st);
+    return launch(q8_row_kernel<MODE, TX, TY, V, NV, false>, (unsigned)p.rows, (unsigned)threads, 0, p, st);
+}
+
+// Threads per row. Many rows: 32 or 16 values a thread (whichever leaves fewer of the row's threads idle; loads in flight are what counts).
+// Few rows: as many threads as there are vectors, so that a row costs one load's latency and two reductions.
+template <int MODE, typename TX, typename TY, int V> int launch_vec(const RowArgs& p, cudaStream_t st) {
+    const int vecs = (p.C + V - 1) / V;
+    constexpr int MOST = V == 1 ? 16 : 32 / V;   // accesses per thread (single elements: 16, or a block could not have 512 threads)
+    const auto threads_for = [&](int n) { return ((vecs + n - 1) / n + 31) / 32 * 32; };
+    int nv = MOST;
+    if (threads_for(nv / 2) <= 512 && threads_for(nv / 2) * (nv / 2) < threads_for(nv) * nv) nv /= 2;
+    while (nv > 1 && threads_for(nv / 2) <= 512 && (long)p.rows * threads_for(nv) < 148L * 512) nv /= 2;
+    const int threads = threads_for(nv);
+    if constexpr (MOST >= 16) {
+        if (nv > 8) return launch_rows<MODE, TX, TY, V, 16>(p, threads, st);
+    }
+    if constexpr (MOST >= 8) {
+        if (nv > 4) return launch_rows<MODE, TX, TY, V, 8>(p, threads, st);
+    }
+    if (nv > 2) return launch_rows<MODE, TX, TY, V, 4>(p, threads, st);
+    if (nv > 1) return launch_rows<MODE, TX, TY, V, 2>(p, threads, st);
+    return launch_rows<MODE, TX, TY, V, 1>(p, threads, st);
+}
+
+template <int MODE, typename TX, typename TY> int run_rows(const RowArgs& p, cudaStream_t st) {
+    constexpr int V = 16 / (int)sizeof(TX);
+    constexpr int SCALAR_MOST = 16 * 512, VEC_MOST = 32 * 512;
+    const auto wide = [&]() {
+        static std::atomic<unsigned long long> done{0};
+        if (first_use_on_current_device(done))
+            if (cudaFuncSetAttribute(q8_wide_row_kernel<MODE, TX, TY>, cudaFuncAttributeMaxDynamicSharedMemorySize, Q8_MAX_COLUMNS * 4) != cudaSuccess) return -5;
+        return launch(q8_wide_row_kernel<MODE, TX, TY>, (unsigned)p.rows, 1024, (size_t)p.C * 4, p, st);
+    };
+    // Vectors of 16 bytes of x, and as many elements of everything else, where every row of every operand starts on such a boundary.
+    const auto fits = [](const void* ptr, int ld, size_t elem) { return ((uintptr_t)ptr % (V * elem > 16 ? 16 : V * elem)) == 0 && (ld % V) == 0; };
+    const bool vec = (p.C % V) == 0 && fits(p.x, p.ldx, sizeof(TX)) && fits(p.q, p.ldq, 1) && (!p.y || fits(p.y, p.ldy, sizeof(TY))) &&
+                     (!p.sum || fits(p.sum, p.lds, sizeof(TX))) && (!p.w || fits(p.w, V, sizeof(float)));
+    if (p.C > (vec ? VEC_MOST : SCALAR_MOST)) return wide();
+    return vec ? launch_vec<MODE, TX, TY, V>(p, st) : launch_vec<MODE, TX, TY, 1>(p, st);
 }
 
 }  // namespace
 
 int q8_quantize_rows(int dtype, int8_t* q, int ldq, float* scale, const void* x, int ldx, int rows, int C, cudaStream_t st) {
-    RowArgs p{q, scale, x, nullptr, nullptr, nullptr, ldq, ldx, 0, 0, C, 0.0f};
-    return dtype ? launch<Q8_ROWS, bf16, bf16>(p, rows, st) : launch<Q8_ROWS, float, float>(p, rows, st);
+    RowArgs p{q, scale, x, nullptr, nullptr, nullptr, ldq, ldx, 0, 0, C, rows, 0.0f};
+    return dtype ? run_rows<Q8_ROWS, bf16, bf16>(p, st) : run_rows<Q8_ROWS, float, float>(p, st);
 }
 
 int q8_rmsnorm(int dtype, int8_t* q, int ldq, float* scale, void* sum, int lds, const void* x, int ldx, int add_dtype, const void* add, int lda,
                const float* w, int rows, int C, float eps, cudaStream_t st) {
-    RowArgs p{q, scale, x, add, sum, w, ldq, ldx, lda, lds, C, eps};
-    if (dtype) return add_dtype ? launch<Q8_NORM, bf16, bf16>(p, rows, st) : launch<Q8_NORM, bf16, float>(p, rows, st);
-    return add_dtype ? launch<Q8_NORM, float, bf16>(p, rows, st) : launch<Q8_NORM, float, float>(p, rows, st);
+    RowArgs p{q, scale, x, add, sum, w, ldq, ldx, lda, lds, C, rows, eps};
+    if (dtype) return add_dtype ? run_rows<Q8_NORM, bf16, bf16>(p, st) : run_rows<Q8_NORM, bf16, float>(p, st);
+    return add_dtype ? run_rows<Q8_NORM, float, bf16>(p, st) : run_rows<Q8_NORM, float, float>(p, st);
 }
 
 int q8_swiglu(int dtype, int8_t* q, int ldq, float* scale, const void* gate, const void* up, int ldgu, int rows, int H, cudaStream_t st) {
-    RowArgs p{q, scale, gate, up, nullptr, nullptr, ldq, ldgu, ldgu, 0, H, 0.0f};
-    return dtype ? launch<Q8_SWIGLU, bf16, bf16>(p, rows, st) : launch<Q8_SWIGLU, float, float>(p, rows, st);
+    RowArgs p{q, scale, gate, up, nullptr, nullptr, ldq, ldgu, ldgu, 0, H, rows, 0.0f};
+    return dtype ? run_rows<Q8_SWIGLU, bf16, bf16>(p, st) : run_rows<Q8_SWIGLU, float, float>(p, st);
 }
 
 }  // namespace bmb
