@@ -1,63 +1,491 @@
 // Product of 8-bit integer matrices with a scale per row of each (per token and per output channel):
 //   out[m, n] = (sum_k q[m, k] w[n, k]) * (scale[m] * wscale[n]) (+ residual[m, n])
-// The sum is an exact 32-bit integer for every K up to 131071 (|q w| <= 2^14), so the only roundings are the conversion of the sum, the
-// product of the scales, their product, the residual's addition and the store: the result does not depend on the order of the sum.
+// The sum is an exact 32-bit integer for every K up to 131056 (|q w| <= 2^14), so the only roundings are the conversion of the sum, the
+// product of the scales, their product, the residual's addition and the store: the result does not depend on the order of the sum, and a
+// reduction split over several CTAs is as exact (and as reproducible) as one that is not.
+//
+// Both kernels compute the transposed tile: the weights are the A operand (128 output channels = the 128 lanes of tensor memory), the tokens
+// the B operand (16 to 256 of them = accumulator columns). A warp then holds 32 consecutive channels of one token in one register across
+// its lanes, so that a plain store of that register is a contiguous 128-byte (fp32) or 64-byte (bf16) piece of an output row whatever its
+// alignment, the channel's scale is a register of the lane and the token's a broadcast from shared memory. Few tokens cost a narrow
+// instruction instead of an empty tile.
+//   q8_split_kernel  one tile of 128 channels per cluster; the CTAs of the cluster split K and exchange their partial sums through
+//                    distributed shared memory. For outputs of too few tiles to fill the GPU: decode, short prompts.
+//   q8_pair_kernel   persistent CTA pairs with tiles of 256 channels x up to 256 tokens, for everything larger.
 #include "q8_kernels.cuh"
+
+#include <cuda.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdio>
+#include <cstdlib>
+
+#include "ptx_sm100.cuh"
 
 namespace bmb {
 
 namespace {
 
-constexpr int T = 64, KT = 64;   // tile of the output, and of K per step
+constexpr int BM = 128;                   // channels per CTA
+constexpr int BK = 128;                   // codes per k-block: one 128-byte swizzled row
+constexpr int UK = 32;                    // codes per instruction
+constexpr int A_BYTES = BM * BK;          // 16 KB
+constexpr int NUM_THREADS = 192;          // warp 0 copies, warp 1 issues the products, warps 2 to 5 are the epilogue (lane quarter = warp & 3)
+constexpr int MAX_STAGES = 8;
 
-template <typename TO>
-__global__ void __launch_bounds__(256) q8_matmul_kernel(TO* out, int ldo, const int8_t* q, int ldq, const float* scale, const int8_t* w,
-                                                        const float* wscale, const TO* residual, int ldr, int M, int K, int N, int tiles_n) {
-    __shared__ int sq[T][KT / 4 + 1], sw[T][KT / 4 + 1];
-    const int m0 = (int)(blockIdx.x / tiles_n) * T, n0 = (int)(blockIdx.x % tiles_n) * T;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    int acc[4][4] = {};
-    for (int k0 = 0; k0 < K; k0 += KT) {
-        const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 16;
-        const int4 z = make_int4(0, 0, 0, 0);
-        const int4 a = m0 + r < M && k0 + c < K ? *(const int4*)(q + (size_t)(m0 + r) * ldq + k0 + c) : z;
-        const int4 b = n0 + r < N && k0 + c < K ? *(const int4*)(w + (size_t)(n0 + r) * K + k0 + c) : z;
-        int* da = &sq[r][c / 4];
-        int* db = &sw[r][c / 4];
-        da[0] = a.x; da[1] = a.y; da[2] = a.z; da[3] = a.w;
-        db[0] = b.x; db[1] = b.y; db[2] = b.z; db[3] = b.w;
-        __syncthreads();
-        for (int k = 0; k < KT / 4; ++k)
+struct Q8Args {
+    void* out;
+    const void* residual;
+    const float *scale, *wscale;
+    int ldo, ldr, M, N, K;     // M tokens, N channels
+    int bn;                    // tokens per tile
+    int tiles_ch, tiles_tok, kb_total;
+    int splits, kb_per, stages;   // split kernel
+    int* err;
+};
+
+// One channel (this lane's) of up to 32 consecutive tokens, accumulators r, token scales sa. The residual's values are all read before the
+// first store: out may be the residual.
+template <typename TO> __device__ __forceinline__ void store_tokens(const Q8Args& p, int m, int n, const uint32_t (&r)[32], const float* sa, float sw, int tokens) {
+    TO* o = (TO*)p.out + (size_t)m * p.ldo + n;
+    float f[32];
+    if (p.residual) {
+        const TO* res = (const TO*)p.residual + (size_t)m * p.ldr + n;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(sq[ty + 16 * i][k], sw[tx + 16 * j][k], acc[i][j]);
-        __syncthreads();
+        for (int i = 0; i < 32; ++i) f[i] = i < tokens ? to_f32(res[(size_t)i * p.ldr]) : 0.0f;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 32; ++i) {
+        const float v = (float)(int)r[i] * (sa[i] * sw);
+        if (i < tokens) o[(size_t)i * p.ldo] = from_f32<TO>(p.residual ? v + f[i] : v);
+    }
+}
+// this warp's copy of a tile's token scales
+__device__ __forceinline__ void load_scales(const Q8Args& p, float* sa, int m0, int lane) {
+    for (int j = lane; j < p.bn; j += 32) sa[j] = m0 + j < p.M ? p.scale[m0 + j] : 0.0f;
+    __syncwarp();
+}
+
+// the instructions of one k-block; the last block of K may hold fewer than four (what lies beyond K is zero)
+__device__ __forceinline__ int instructions(const Q8Args& p, int kb) { return min(BK / UK, (p.K - kb * BK + UK - 1) / UK); }
+
+// a wait ran out somewhere in this CTA: let copies and products in flight land before their memory is given back, and say so
+__device__ __forceinline__ void report_abort(const Q8Args& p, volatile int* abort_flag) {
+    if (!*abort_flag) return;
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 2000000ull) __nanosleep(1000);
+    if (threadIdx.x == 0 && p.err) atomicExch(p.err, 3000);
+}
+
+// ---- split-K over a cluster ------------------------------------------------------------------------------------------------------------
+struct __align__(8) SplitBarriers {
+    uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc;
+    uint32_t tmem_base;
+    int abort_flag;
+};
+
+template <typename TO>
+__global__ void __launch_bounds__(NUM_THREADS) q8_split_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmQ, const Q8Args p) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ SplitBarriers bars;
+    __shared__ float s_sa[4][256];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    const int b_bytes = p.bn * BK, stage_bytes = A_BYTES + b_bytes;
+    int* red = (int*)(smem + p.stages * stage_bytes);   // [splits][bn / splits][128]: this CTA's columns of every CTA's partial sums
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int split = p.splits > 1 ? (int)cluster_ctarank() : 0;
+    const int tile = (int)blockIdx.x / p.splits;
+    const int m0 = tile / p.tiles_ch * p.bn, n0 = tile % p.tiles_ch * BM;
+    const int kb0 = split * p.kb_per, kb1 = min(p.kb_total, kb0 + p.kb_per);
+    const uint32_t tmem_cols = p.bn <= 32 ? 32u : p.bn <= 64 ? 64u : p.bn <= 128 ? 128u : 256u;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.stages; ++s) {
+            mbar_init(&bars.full[s], 1);
+            mbar_init(&bars.empty[s], 1);
+        }
+        mbar_init(&bars.acc, 1);
+        bars.abort_flag = 0;
+        mbar_fence_init();
+        fence_proxy_async_smem();
+    }
+    if (warp == 1) {
+        tmem_alloc(&bars.tmem_base, tmem_cols);
+        tmem_relinquish();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (p.splits > 1) cluster_arrive();   // "this CTA runs": its peers may write to its shared memory once all have arrived
+    const uint32_t tmem_base = bars.tmem_base;
+    volatile int* abort_flag = &bars.abort_flag;
+    bool ok = true;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int kb = kb0, i = 0; kb < kb1 && ok; ++kb, ++i) {
+                const int s = i % p.stages;
+                if (i >= p.stages && !mbar_wait(&bars.empty[s], (i / p.stages - 1) & 1, abort_flag)) { ok = false; break; }
+                uint8_t* st = smem + s * stage_bytes;
+                mbar_expect_tx(&bars.full[s], (uint32_t)stage_bytes);
+                tma_load_2d(st, &tmW, &bars.full[s], kb * BK, n0);
+                tma_load_2d(st + A_BYTES, &tmQ, &bars.full[s], kb * BK, m0);
+            }
+            // the CTA may not retire while commits can still arrive on `empty`
+            for (int i = max(0, kb1 - kb0 - p.stages); i < kb1 - kb0 && ok; ++i) ok = mbar_wait(&bars.empty[i % p.stages], (i / p.stages) & 1, abort_flag);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const uint32_t idesc = umma_idesc_s8_s32(BM, p.bn);
+            uint32_t acc = 0;
+            for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
+                const int s = i % p.stages;
+                if (!mbar_wait(&bars.full[s], (i / p.stages) & 1, abort_flag)) { ok = false; break; }
+                tc_fence_after_sync();
+                const uint32_t at = smem_u32(smem + s * stage_bytes);
+                const uint64_t ad = umma_smem_desc_sw128(at, 16, 1024), bd = umma_smem_desc_sw128(at + A_BYTES, 16, 1024);
+                const int n = instructions(p, kb);
+                for (int k = 0; k < n; ++k, acc = 1) umma_s8_ss(tmem_base, ad + 2 * k, bd + 2 * k, idesc, acc);
+                umma_commit(&bars.empty[s]);
+            }
+            if (ok) umma_commit(&bars.acc);
+        }
+        __syncwarp();
+    } else {
+        const int qd = warp & 3, n = n0 + qd * 32 + lane;
+        float* sa = s_sa[qd];
+        load_scales(p, sa, m0, lane);
+        const float sw = n < p.N ? p.wscale[n] : 0.0f;
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars.acc, 0, abort_flag));
+        if (ok) {
+            tc_fence_after_sync();
+            if (p.splits == 1)
+                for (int c0 = 0; c0 < p.bn && m0 + c0 < p.M; c0 += 32) {
+                    uint32_t r[32];
+                    tmem_ld_32x32(tmem_base + ((uint32_t)(qd * 32) << 16) + c0, r);
+                    tmem_ld_wait();
+                    if (n < p.N) store_tokens<TO>(p, m0 + c0, n, r, sa + c0, sw, min(min(32, p.bn - c0), p.M - m0 - c0));
+                    __syncwarp();
+                }
+        }
+    }
+    if (p.splits > 1) {
+        // every CTA of the cluster owns bn / splits columns: partial sums go to their owners, who add and store them
+        const int own = p.bn / p.splits, qd = warp & 3;
+        cluster_wait();
+        if (warp >= 2 && ok) {
+            for (int c0 = 0; c0 < p.bn; c0 += 32) {
+                uint32_t r[32];
+                tmem_ld_32x32(tmem_base + ((uint32_t)(qd * 32) << 16) + c0, r);
+                tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-            if (m < M && n < N) {
-                float f = (float)acc[i][j] * (scale[m] * wscale[n]);
-                if (residual) f += to_f32(residual[(size_t)m * ldr + n]);
-                out[(size_t)m * ldo + n] = from_f32<TO>(f);
+                for (int i = 0; i < 32; ++i) {
+                    const int c = c0 + i, owner = c / own;
+                    if (c < p.bn) st_cluster_u32(mapa_shared(red + (split * own + c - owner * own) * BM + qd * 32 + lane, (uint32_t)owner), r[i]);
+                }
             }
         }
+        __syncwarp();
+        cluster_sync_all();
+        const int n = n0 + qd * 32 + lane, m = m0 + split * own;
+        if (warp >= 2 && n < p.N) {
+            const float sw = p.wscale[n];
+            for (int c0 = 0; c0 < own && m + c0 < p.M; c0 += 32) {
+                uint32_t r[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    r[i] = 0;
+                    if (c0 + i < own)
+                        for (int s = 0; s < p.splits; ++s) r[i] += (uint32_t)red[(s * own + c0 + i) * BM + qd * 32 + lane];
+                }
+                store_tokens<TO>(p, m + c0, n, r, s_sa[qd] + split * own + c0, sw, min(min(32, own - c0), p.M - m - c0));
+            }
+        }
+    }
+    __syncwarp();
+    report_abort(p, abort_flag);
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    if (warp == 1) tmem_dealloc(tmem_base, tmem_cols);
+}
+
+// ---- persistent CTA pairs --------------------------------------------------------------------------------------------------------------
+constexpr int PAIR_STAGES = 3, KPS = 2;                     // a ring stage holds two k-blocks: one wait and one commit for eight instructions
+constexpr int PAIR_STAGE_BYTES = KPS * 2 * A_BYTES;         // this CTA's 128 channels and its half (at most 128) of the tokens
+constexpr int PAIR_SMEM = PAIR_STAGES * PAIR_STAGE_BYTES + 1024;
+
+struct __align__(8) PairBarriers {
+    uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], acc_full[2], acc_empty[2];
+    uint32_t tmem_base;
+    int abort_flag;
+};
+
+// Channel tiles run fastest inside groups of RASTER of them, so that a wave of pairs shares its tokens and one group's weights stay in L2.
+constexpr int RASTER = 32;
+__device__ __forceinline__ void pair_tile(const Q8Args& p, int u, int& m0, int& n0) {
+    const int per_group = RASTER * p.tiles_tok;
+    const int g = u / per_group, idx = u - g * per_group, w = min(RASTER, p.tiles_ch - g * RASTER);
+    const int tt = idx / w;
+    m0 = tt * p.bn;
+    n0 = (g * RASTER + idx - tt * w) * 2 * BM;
+}
+
+template <typename TO>
+__global__ void __launch_bounds__(NUM_THREADS, 1) q8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmQ, const Q8Args p) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ PairBarriers bars;
+    __shared__ float s_sa[4][256];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    const uint32_t rank = cluster_ctarank();
+    const int worker = blockIdx.x >> 1, nworkers = gridDim.x >> 1;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int units = p.tiles_ch * p.tiles_tok, half = p.bn / 2;
+    const int b_bytes = half * BK, st_bytes = KPS * (A_BYTES + b_bytes);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < PAIR_STAGES; ++s) {
+            mbar_init(&bars.full[s], 1);    // the leader's is used; both CTAs' copies count their bytes on it
+            mbar_init(&bars.empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&bars.acc_full[b], 1);
+            mbar_init(&bars.acc_empty[b], 8);   // the leader's collects the epilogue warps of both CTAs
+        }
+        bars.abort_flag = 0;
+        mbar_fence_init();
+        fence_proxy_async_smem();
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(&bars.tmem_base, 512);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync_all();   // the peer's barriers exist before anything is signalled across the pair
+    tc_fence_after_sync();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const uint32_t tmem_base = bars.tmem_base;
+    volatile int* abort_flag = &bars.abort_flag;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            tma_prefetch_desc(&tmW);
+            tma_prefetch_desc(&tmQ);
+            int s = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int u = worker; u < units && ok; u += nworkers) {
+                int m0, n0;
+                pair_tile(p, u, m0, n0);
+                n0 += (int)rank * BM;
+                m0 += (int)rank * half;
+                for (int kb = 0; kb < p.kb_total; kb += KPS, s = (s + 1 == PAIR_STAGES ? 0 : s + 1), ph ^= (s == 0)) {
+                    if (!mbar_wait(&bars.empty[s], ph ^ 1, abort_flag)) { ok = false; break; }
+                    const int g = min(KPS, p.kb_total - kb);
+                    uint8_t* st = smem + s * st_bytes;
+                    const uint32_t full = mapa_shared(&bars.full[s], 0);
+                    if (rank == 0) mbar_expect_tx(&bars.full[s], (uint32_t)(2 * g * (A_BYTES + b_bytes)));
+                    for (int j = 0; j < g; ++j) {
+                        tma_load_2d_pair(st + j * A_BYTES, &tmW, full, (kb + j) * BK, n0);
+                        tma_load_2d_pair(st + KPS * A_BYTES + j * b_bytes, &tmQ, full, (kb + j) * BK, m0);
+                    }
+                }
+            }
+            // the CTA may not retire while commits can still arrive on `empty`
+            for (int i = 0; i < PAIR_STAGES && ok; ++i, s = (s + 1 == PAIR_STAGES ? 0 : s + 1), ph ^= (s == 0))
+                if (!mbar_wait(&bars.empty[s], ph ^ 1, abort_flag)) ok = false;
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            const uint32_t idesc = umma_idesc_s8_s32(2 * BM, p.bn);
+            const uint64_t ad0 = umma_smem_desc_sw128(smem_u32(smem), 16, 1024), bd0 = umma_smem_desc_sw128(smem_u32(smem + KPS * A_BYTES), 16, 1024);
+            int s = 0, it = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int u = worker; u < units && ok; u += nworkers, ++it) {
+                const int buf = it & 1;
+                if (!mbar_wait(&bars.acc_empty[buf], ((it >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                tc_fence_after_sync();
+                uint32_t acc = 0;
+                for (int kb = 0; kb < p.kb_total; kb += KPS) {
+                    if (!mbar_wait(&bars.full[s], ph, abort_flag)) { ok = false; break; }
+                    tc_fence_after_sync();
+                    const int g = min(KPS, p.kb_total - kb);
+                    for (int j = 0; j < g; ++j) {
+                        uint64_t ad = ad0 + (uint32_t)((s * st_bytes + j * A_BYTES) >> 4), bd = bd0 + (uint32_t)((s * st_bytes + j * b_bytes) >> 4);
+                        const int n = instructions(p, kb + j);
+                        if (n == BK / UK) {
+#pragma unroll
+                            for (int k = 0; k < BK / UK; ++k, ad += 2, bd += 2, acc = 1) umma_s8_ss_pair(tmem_base + buf * 256, ad, bd, idesc, acc);
+                        } else {
+                            for (int k = 0; k < n; ++k, ad += 2, bd += 2, acc = 1) umma_s8_ss_pair(tmem_base + buf * 256, ad, bd, idesc, acc);
+                        }
+                    }
+                    umma_commit_pair(&bars.empty[s], 3);
+                    if (++s == PAIR_STAGES) { s = 0; ph ^= 1u; }
+                }
+                if (ok) umma_commit_pair(&bars.acc_full[buf], 3);
+            }
+        }
+    } else {
+        const int qd = warp & 3;
+        float* sa = s_sa[qd];
+        int it = 0;
+        for (int u = worker; u < units; u += nworkers, ++it) {
+            int m0, n0;
+            pair_tile(p, u, m0, n0);
+            const int buf = it & 1, n = n0 + (int)rank * BM + qd * 32 + lane;
+            load_scales(p, sa, m0, lane);
+            const float sw = n < p.N ? p.wscale[n] : 0.0f;
+            if (!__all_sync(0xffffffffu, mbar_wait(&bars.acc_full[buf], (it >> 1) & 1, abort_flag))) break;
+            tc_fence_after_sync();
+            const uint32_t t0 = tmem_base + ((uint32_t)(qd * 32) << 16) + (uint32_t)(buf * 256);
+            for (int c0 = 0; c0 < p.bn && m0 + c0 < p.M; c0 += 32) {
+                uint32_t r[32];
+                tmem_ld_32x32(t0 + c0, r);
+                tmem_ld_wait();
+                if (n < p.N) store_tokens<TO>(p, m0 + c0, n, r, sa + c0, sw, min(32, p.M - m0 - c0));
+                __syncwarp();
+            }
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+                if (rank != 0) mbar_arrive_cluster(mapa_shared(&bars.acc_empty[buf], 0));
+                else mbar_arrive(&bars.acc_empty[buf]);
+            }
+        }
+    }
+    __syncwarp();
+    report_abort(p, abort_flag);
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync_all();   // no signal of the peer may still be on its way to this CTA's barriers
+    tc_fence_after_sync();
+    if (warp == 1) tmem_dealloc_pair(tmem_base, 512);
+}
+
+// ---- launch ----------------------------------------------------------------------------------------------------------------------------
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// codes[rows][K] at a pitch of `ld` bytes, in boxes of box_rows rows x one k-block, 128-byte swizzle, zeros outside
+bool code_map(CUtensorMap* tm, const void* base, int K, int rows, int64_t ld, int box_rows) {
+    static const EncodeTiledFn fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess ? (EncodeTiledFn)f : nullptr;
+    }();
+    const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld};
+    const cuuint32_t box[2] = {BK, (cuuint32_t)box_rows}, step[2] = {1, 1};
+    return fn && fn(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int ceil_div(int a, int b) { return a / b + (a % b != 0); }
+
+constexpr int SPLIT_RING = 96 * 1024;   // two CTAs of the split kernel fit on an SM
+int split_stages(int bn, int kb_per) {
+    const int fit = SPLIT_RING / (A_BYTES + bn * BK);
+    return std::min(std::min(fit, MAX_STAGES), kb_per);
+}
+int split_smem(int bn, int splits, int kb_per) { return split_stages(bn, kb_per) * (A_BYTES + bn * BK) + (splits > 1 ? bn * BM * 4 : 0) + 1024; }
+
+struct Plan {
+    bool pair;
+    int bn, splits;
+};
+
+// Estimated cycles of every tile shape; the smallest is taken.
+Plan choose(int M, int N, int K, int sms) {
+    const int kb = ceil_div(K, BK);
+    Plan best{false, 16, 1};
+    double least = 1e30;
+    for (int bn = 16; bn <= 256; bn *= 2) {
+        if (bn > 16 && bn / 2 >= M) break;
+        for (int s = 1; s <= 8 && (s == 1 || bn <= 128); s *= 2) {
+            const int per = ceil_div(kb, s);
+            if ((s - 1) * per >= kb) continue;
+            const double ctas = (double)ceil_div(N, BM) * ceil_div(M, bn) * s;
+            const double block = std::max((A_BYTES + bn * BK) / 50.0, 4.0 * std::max(60.0, bn / 2.0));
+            const double one = per * block + 10.0 * bn / s + (s > 1 ? 800 + 12.0 * bn : 0.0) + 800;
+            const double t = 2500 + std::ceil(ctas / sms) * one;
+            if (t < least) { least = t; best = Plan{false, bn, s}; }
+        }
+    }
+    for (int bn = 64; bn <= 256; bn += 32) {
+        const double units = (double)ceil_div(N, 2 * BM) * ceil_div(M, bn);
+        const double block = std::max((A_BYTES + bn * BK / 2) / 64.0, std::max(330.0, 2.0 * bn));
+        const double t = 3500 + std::ceil(units / (sms / 2)) * std::max(kb * block, 10.0 * bn) + 10.0 * bn;
+        if (t < least) { least = t; best = Plan{true, bn, 1}; }
+    }
+    return best;
+}
+
+template <typename TO> int launch(Q8Args p, const int8_t* q, int ldq, const int8_t* w, cudaStream_t st) {
+    static std::atomic<unsigned long long> done{0};
+    if (first_use_on_current_device(done)) {
+        if (cudaFuncSetAttribute(q8_pair_kernel<TO>, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM) != cudaSuccess) return -5;
+        if (cudaFuncSetAttribute(q8_split_kernel<TO>, cudaFuncAttributeMaxDynamicSharedMemorySize, split_smem(128, 2, MAX_STAGES)) != cudaSuccess) return -5;
+    }
+    const int sms = sm_count_current_device();
+    Plan plan = choose(p.M, p.N, p.K, sms);
+    if (const char* e = getenv("Q8_PLAN")) { int a, b, c; if (sscanf(e, "%d,%d,%d", &a, &b, &c) == 3) plan = Plan{a != 0, b, c}; }
+    if (getenv("Q8_SAY")) fprintf(stderr, "plan pair %d bn %d splits %d\n", plan.pair, plan.bn, plan.splits);
+    static const bool overlap = getenv("BM_NO_PDL") == nullptr;
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(NUM_THREADS);
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = overlap ? 2 : 1;
+    CUtensorMap tmW, tmQ;
+    p.bn = plan.bn;
+    p.kb_total = ceil_div(p.K, BK);
+    p.tiles_tok = ceil_div(p.M, plan.bn);
+    p.tiles_ch = ceil_div(p.N, plan.pair ? 2 * BM : BM);
+    if (!code_map(&tmW, w, p.K, p.N, p.K, BM) || !code_map(&tmQ, q, p.K, p.M, ldq, plan.pair ? plan.bn / 2 : plan.bn)) return -11;
+    const int64_t tiles = (int64_t)p.tiles_ch * p.tiles_tok;
+    cudaError_t e;
+    if (plan.pair) {
+        if (tiles > 0x3fffffff) return -1;
+        at[0].val.clusterDim.x = 2;
+        cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, sms / 2)));
+        cfg.dynamicSmemBytes = PAIR_SMEM;
+        e = cudaLaunchKernelEx(&cfg, q8_pair_kernel<TO>, tmW, tmQ, p);
+    } else {
+        if (tiles * plan.splits > 0x7fffffff) return -1;
+        p.splits = plan.splits;
+        p.kb_per = ceil_div(p.kb_total, plan.splits);
+        p.stages = split_stages(plan.bn, p.kb_per);
+        at[0].val.clusterDim.x = (unsigned)plan.splits;
+        cfg.gridDim = dim3((unsigned)(tiles * plan.splits));
+        cfg.dynamicSmemBytes = (size_t)split_smem(plan.bn, plan.splits, p.kb_per);
+        e = cudaLaunchKernelEx(&cfg, q8_split_kernel<TO>, tmW, tmQ, p);
+    }
+    if (e == cudaSuccess) return 0;
+    cudaGetLastError();   // a launch that failed must not poison the status of later calls
+    return -9;
 }
 
 }  // namespace
 
 int q8_matmul(int dtype, void* out, int ldo, const int8_t* q, int ldq, const float* scale, const int8_t* w, const float* wscale, const void* residual,
               int ldr, int M, int K, int N, int* err, cudaStream_t st) {
-    (void)err;
-    const int tiles_n = (N + T - 1) / T;
-    const long tiles = (long)((M + T - 1) / T) * tiles_n;
-    if (tiles > 0x7fffffffL) return -1;
-    if (dtype) q8_matmul_kernel<bf16><<<(unsigned)tiles, 256, 0, st>>>((bf16*)out, ldo, q, ldq, scale, w, wscale, (const bf16*)residual, ldr, M, K, N, tiles_n);
-    else q8_matmul_kernel<float><<<(unsigned)tiles, 256, 0, st>>>((float*)out, ldo, q, ldq, scale, w, wscale, (const float*)residual, ldr, M, K, N, tiles_n);
-    return cudaGetLastError() == cudaSuccess ? 0 : -9;
+    if (M > 0x7fffff00 || N > 0x7fffff00) return -1;   // tile origins are 32-bit
+    Q8Args p = {};
+    p.out = out; p.residual = residual; p.scale = scale; p.wscale = wscale;
+    p.ldo = ldo; p.ldr = ldr; p.M = M; p.N = N; p.K = K; p.err = err;
+    return dtype ? launch<bf16>(p, q, ldq, w, st) : launch<float>(p, q, ldq, w, st);
 }
 
 }  // namespace bmb
