@@ -162,15 +162,28 @@ __device__ __forceinline__ uint32_t mapa_shared(const void* p, uint32_t rank) {
 __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// the two halves of it: every thread of every CTA of the cluster arrives once and waits once
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ void st_cluster_u32(uint32_t cluster_addr, uint32_t v) {
-    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+// 16 bytes of shared memory of CTA `rank` of the cluster, at the address `own_addr` has in this CTA
+__device__ __forceinline__ int4 ld_cluster_v4(uint32_t own_addr, uint32_t rank) {
+    int4 v;
+    asm volatile(
+        "{\n\t"
+        ".reg .b32 a;\n\t"
+        "mapa.shared::cluster.u32 a, %4, %5;\n\t"
+        "ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [a];\n\t"
+        "}\n"
+        : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+        : "r"(own_addr), "r"(rank)
+        : "memory");
+    return v;
 }
 // arrive on an mbarrier of another CTA of the cluster (address from mapa_shared)
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// The same without release semantics: it does not wait for the thread's earlier stores to be performed at cluster scope. For a barrier that
+// only says "tensor memory has been read" (tcgen05.wait::ld and tcgen05.fence order that).
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 // Tiled 2-D load into THIS CTA's shared memory whose bytes are counted on an mbarrier given by its shared::cluster
 // address (the pair leader's barrier). No multicast: each CTA fetches its own tile.

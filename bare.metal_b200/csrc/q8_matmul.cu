@@ -31,7 +31,7 @@ constexpr int BM = 128;                   // channels per CTA
 constexpr int BK = 128;                   // codes per k-block: one 128-byte swizzled row
 constexpr int UK = 32;                    // codes per instruction
 constexpr int A_BYTES = BM * BK;          // 16 KB
-constexpr int NUM_THREADS = 192;          // warp 0 copies, warp 1 issues the products, warps 2 to 5 are the epilogue (lane quarter = warp & 3)
+constexpr int NUM_THREADS = 192;          // split kernel: warp 0 copies, warp 1 issues the products, warps 2 to 5 are the epilogue (lane quarter = warp & 3)
 constexpr int MAX_STAGES = 8;
 
 struct Q8Args {
@@ -46,19 +46,35 @@ struct Q8Args {
 };
 
 // One channel (this lane's) of up to 32 consecutive tokens, accumulators r, token scales sa. The residual's values are all read before the
-// first store: out may be the residual.
-template <typename TO> __device__ __forceinline__ void store_tokens(const Q8Args& p, int m, int n, const uint32_t (&r)[32], const float* sa, float sw, int tokens) {
+// first store: out may be the residual. Straight code for whole chunks: with a bound per token the compiler made 21 instructions of each.
+template <typename TO, bool RES> __device__ __forceinline__ void store_tokens(const Q8Args& p, int m, int n, const uint32_t (&r)[32], const float* sa, float sw, int tokens) {
     TO* o = (TO*)p.out + (size_t)m * p.ldo + n;
+    const size_t step = p.ldo;
     float f[32];
-    if (p.residual) {
+    if (RES) {
         const TO* res = (const TO*)p.residual + (size_t)m * p.ldr + n;
+        const size_t rstep = p.ldr;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) f[i] = i < tokens ? to_f32(res[(size_t)i * p.ldr]) : 0.0f;
+        for (int i = 0; i < 32; ++i, res += rstep) f[i] = i < tokens ? to_f32(*res) : 0.0f;
     }
+    if (tokens >= 32) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        const float v = (float)(int)r[i] * (sa[i] * sw);
-        if (i < tokens) o[(size_t)i * p.ldo] = from_f32<TO>(p.residual ? v + f[i] : v);
+        for (int i = 0; i < 32; i += 4) {
+            const float4 s = *(const float4*)(sa + i);
+            const float t[4] = {s.x * sw, s.y * sw, s.z * sw, s.w * sw};
+#pragma unroll
+            for (int j = 0; j < 4; ++j, o += step) {
+                const float v = (float)(int)r[i + j] * t[j];
+                *o = from_f32<TO>(RES ? v + f[i + j] : v);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i, o += step) {
+            if (i >= tokens) break;
+            const float v = (float)(int)r[i] * (sa[i] * sw);
+            *o = from_f32<TO>(RES ? v + f[i] : v);
+        }
     }
 }
 // this warp's copy of a tile's token scales
@@ -85,14 +101,14 @@ struct __align__(8) SplitBarriers {
     int abort_flag;
 };
 
-template <typename TO>
+template <typename TO, bool RES>
 __global__ void __launch_bounds__(NUM_THREADS) q8_split_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmQ, const Q8Args p) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ SplitBarriers bars;
-    __shared__ float s_sa[4][256];
+    __shared__ __align__(16) float s_sa[4][256];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const int b_bytes = p.bn * BK, stage_bytes = A_BYTES + b_bytes;
-    int* red = (int*)(smem + p.stages * stage_bytes);   // [splits][bn / splits][128]: this CTA's columns of every CTA's partial sums
+    int* red = (int*)(smem + p.stages * stage_bytes);   // [bn][128]: this CTA's partial sums
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int split = p.splits > 1 ? (int)cluster_ctarank() : 0;
     const int tile = (int)blockIdx.x / p.splits;
@@ -119,7 +135,6 @@ __global__ void __launch_bounds__(NUM_THREADS) q8_split_kernel(const __grid_cons
     tc_fence_after_sync();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (p.splits > 1) cluster_arrive();   // "this CTA runs": its peers may write to its shared memory once all have arrived
     const uint32_t tmem_base = bars.tmem_base;
     volatile int* abort_flag = &bars.abort_flag;
     bool ok = true;
@@ -149,7 +164,9 @@ __global__ void __launch_bounds__(NUM_THREADS) q8_split_kernel(const __grid_cons
                 const uint32_t at = smem_u32(smem + s * stage_bytes);
                 const uint64_t ad = umma_smem_desc_sw128(at, 16, 1024), bd = umma_smem_desc_sw128(at + A_BYTES, 16, 1024);
                 const int n = instructions(p, kb);
-                for (int k = 0; k < n; ++k, acc = 1) umma_s8_ss(tmem_base, ad + 2 * k, bd + 2 * k, idesc, acc);
+#pragma unroll
+                for (int k = 0; k < BK / UK; ++k, acc = 1)
+                    if (k < n) umma_s8_ss(tmem_base, ad + 2 * k, bd + 2 * k, idesc, acc);
                 umma_commit(&bars.empty[s]);
             }
             if (ok) umma_commit(&bars.acc);
@@ -168,43 +185,54 @@ __global__ void __launch_bounds__(NUM_THREADS) q8_split_kernel(const __grid_cons
                     uint32_t r[32];
                     tmem_ld_32x32(tmem_base + ((uint32_t)(qd * 32) << 16) + c0, r);
                     tmem_ld_wait();
-                    if (n < p.N) store_tokens<TO>(p, m0 + c0, n, r, sa + c0, sw, min(min(32, p.bn - c0), p.M - m0 - c0));
+                    if (n < p.N) store_tokens<TO, RES>(p, m0 + c0, n, r, sa + c0, sw, min(min(32, p.bn - c0), p.M - m0 - c0));
                     __syncwarp();
                 }
         }
     }
     if (p.splits > 1) {
-        // every CTA of the cluster owns bn / splits columns: partial sums go to their owners, who add and store them
+        // Partial sums into this CTA's shared memory, then every CTA adds bn / splits of the columns over the cluster: a warp takes a token,
+        // a lane four channels of it, 16 bytes from each CTA.
         const int own = p.bn / p.splits, qd = warp & 3;
-        cluster_wait();
         if (warp >= 2 && ok) {
             for (int c0 = 0; c0 < p.bn; c0 += 32) {
                 uint32_t r[32];
                 tmem_ld_32x32(tmem_base + ((uint32_t)(qd * 32) << 16) + c0, r);
                 tmem_ld_wait();
+                int* to = red + c0 * BM + qd * 32 + lane;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const int c = c0 + i, owner = c / own;
-                    if (c < p.bn) st_cluster_u32(mapa_shared(red + (split * own + c - owner * own) * BM + qd * 32 + lane, (uint32_t)owner), r[i]);
-                }
+                for (int i = 0; i < 32; ++i)
+                    if (i < 16 || p.bn > 16) to[i * BM] = (int)r[i];
             }
         }
         __syncwarp();
         cluster_sync_all();
-        const int n = n0 + qd * 32 + lane, m = m0 + split * own;
-        if (warp >= 2 && n < p.N) {
-            const float sw = p.wscale[n];
-            for (int c0 = 0; c0 < own && m + c0 < p.M; c0 += 32) {
-                uint32_t r[32];
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    r[i] = 0;
-                    if (c0 + i < own)
-                        for (int s = 0; s < p.splits; ++s) r[i] += (uint32_t)red[(s * own + c0 + i) * BM + qd * 32 + lane];
+        if (warp >= 2) {
+            const int n = n0 + 4 * lane;
+            for (int c = qd; c < own; c += 4) {
+                const int j = split * own + c, m = m0 + j;
+                if (m >= p.M || n >= p.N) break;
+                const uint32_t at = smem_u32(red + j * BM + 4 * lane);
+                int4 sum = make_int4(0, 0, 0, 0);
+#pragma unroll 4
+                for (int s = 0; s < p.splits; ++s) {
+                    const int4 v = ld_cluster_v4(at, (uint32_t)s);
+                    sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
                 }
-                store_tokens<TO>(p, m + c0, n, r, s_sa[qd] + split * own + c0, sw, min(min(32, own - c0), p.M - m - c0));
+                const int part[4] = {sum.x, sum.y, sum.z, sum.w};
+                const float sa = s_sa[qd][j];
+                TO* o = (TO*)p.out + (size_t)m * p.ldo + n;
+                const TO* res = RES ? (const TO*)p.residual + (size_t)m * p.ldr + n : nullptr;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (n + i < p.N) {
+                        const float v = (float)part[i] * (sa * p.wscale[n + i]);
+                        o[i] = from_f32<TO>(RES ? v + to_f32(res[i]) : v);
+                    }
             }
         }
+        __syncwarp();
+        cluster_sync_all();   // nobody leaves while its shared memory is still read
     }
     __syncwarp();
     report_abort(p, abort_flag);
@@ -215,54 +243,91 @@ __global__ void __launch_bounds__(NUM_THREADS) q8_split_kernel(const __grid_cons
 }
 
 // ---- persistent CTA pairs --------------------------------------------------------------------------------------------------------------
-constexpr int PAIR_STAGES = 3, KPS = 2;                     // a ring stage holds two k-blocks: one wait and one commit for eight instructions
-constexpr int PAIR_STAGE_BYTES = KPS * 2 * A_BYTES;         // this CTA's 128 channels and its half (at most 128) of the tokens
-constexpr int PAIR_SMEM = PAIR_STAGES * PAIR_STAGE_BYTES + 1024;
+// HELD = false: both operands stream through the ring, tiles of 256 channels x bn tokens in raster order.
+// HELD = true (K of at most HELD_BLOCKS k-blocks): a tile's weights stay in shared memory while the pair walks the tokens, so that a tile
+// moves half the bytes. With both operands streaming, every k-block of a 256 x 256 tile brings 32 KB to each SM for 512 cycles of products,
+// and the L2 gives an SM about 43 bytes per cycle when all of them ask: 760 cycles per k-block at any K.
+constexpr int KPS = 2;                    // k-blocks per ring stage: one wait and one commit for eight instructions
+constexpr int PAIR_STAGES = 3;
+constexpr int HELD_BLOCKS = 8;
+constexpr int HELD_BN = 224;              // widest token tile whose ring fits beside 128 KB of weights
+constexpr int EPI_WARPS = 8;              // two per lane quarter, taking 32-token chunks in turn
+constexpr int PAIR_THREADS = 96 + 32 * EPI_WARPS;   // warps 0 and 1 copy, warp 2 issues the products
+constexpr int PAIR_SMEM = PAIR_STAGES * KPS * 2 * A_BYTES + 1024;
+constexpr int HELD_SMEM = HELD_BLOCKS * A_BYTES + PAIR_STAGES * KPS * (HELD_BN / 2) * BK + 1024;
 
 struct __align__(8) PairBarriers {
-    uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], acc_full[2], acc_empty[2];
+    uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], acc_full[2], acc_empty[2], held_full, held_empty;
     uint32_t tmem_base;
     int abort_flag;
 };
 
-// Channel tiles run fastest inside groups of RASTER of them, so that a wave of pairs shares its tokens and one group's weights stay in L2.
+// The units of one pair, in order. Streaming: round-robin over the pairs; channel tiles run fastest inside groups of RASTER of them, so that
+// a wave shares its tokens and one group's weights stay in L2. Held: a contiguous run of units, tokens fastest.
 constexpr int RASTER = 32;
-__device__ __forceinline__ void pair_tile(const Q8Args& p, int u, int& m0, int& n0) {
-    const int per_group = RASTER * p.tiles_tok;
-    const int g = u / per_group, idx = u - g * per_group, w = min(RASTER, p.tiles_ch - g * RASTER);
-    const int tt = idx / w;
-    m0 = tt * p.bn;
-    n0 = (g * RASTER + idx - tt * w) * 2 * BM;
-}
+template <bool HELD> struct Units {
+    int u, end, step;
+    __device__ __forceinline__ Units(const Q8Args& p, int worker, int workers) {
+        const int64_t all = (int64_t)p.tiles_ch * p.tiles_tok;
+        u = HELD ? (int)(all * worker / workers) : worker;
+        end = HELD ? (int)(all * (worker + 1) / workers) : (int)all;
+        step = HELD ? 1 : workers;
+    }
+    __device__ __forceinline__ bool more() const { return u < end; }
+    __device__ __forceinline__ void next() { u += step; }
+    // first channel and token of the unit
+    __device__ __forceinline__ void tile(const Q8Args& p, int& n0, int& m0) const {
+        if (HELD) {
+            const int c = u / p.tiles_tok;
+            n0 = c * 2 * BM;
+            m0 = (u - c * p.tiles_tok) * p.bn;
+            return;
+        }
+        const int per_group = RASTER * p.tiles_tok;
+        const int g = u / per_group, idx = u - g * per_group, w = min(RASTER, p.tiles_ch - g * RASTER);
+        const int t = idx / w;
+        m0 = t * p.bn;
+        n0 = (g * RASTER + idx - t * w) * 2 * BM;
+    }
+};
 
-template <typename TO>
-__global__ void __launch_bounds__(NUM_THREADS, 1) q8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmQ, const Q8Args p) {
+template <typename TO, bool RES, bool HELD>
+__global__ void __launch_bounds__(PAIR_THREADS, 1) q8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmQ, const Q8Args p) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ PairBarriers bars;
-    __shared__ float s_sa[4][256];
+    __shared__ __align__(16) float s_sa[EPI_WARPS][128];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const uint32_t rank = cluster_ctarank();
-    const int worker = blockIdx.x >> 1, nworkers = gridDim.x >> 1;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int units = p.tiles_ch * p.tiles_tok, half = p.bn / 2;
-    const int b_bytes = half * BK, st_bytes = KPS * (A_BYTES + b_bytes);
+    const int worker = blockIdx.x >> 1, workers = gridDim.x >> 1;
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;   // uniform for the compiler, too
+    const int half = p.bn / 2, b_bytes = half * BK;
+    // HELD: [8 k-blocks of weights][ring of tokens]; otherwise a ring of [2 k-blocks of weights][2 k-blocks of tokens]
+    const int st_bytes = KPS * (HELD ? b_bytes : A_BYTES + b_bytes);
+    uint8_t* ring = smem + (HELD ? HELD_BLOCKS * A_BYTES : 0);
+    const int b_at = HELD ? 0 : KPS * A_BYTES;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < PAIR_STAGES; ++s) {
-            mbar_init(&bars.full[s], 1);    // the leader's is used; both CTAs' copies count their bytes on it
+            mbar_init(&bars.full[s], 2);    // the leader's is used, by its two producers; both CTAs' copies count their bytes on it
             mbar_init(&bars.empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&bars.acc_full[b], 1);
-            mbar_init(&bars.acc_empty[b], 8);   // the leader's collects the epilogue warps of both CTAs
+            mbar_init(&bars.acc_empty[b], 2 * EPI_WARPS);   // the leader's collects the epilogue warps of both CTAs
         }
+        mbar_init(&bars.held_full, 2);
+        mbar_init(&bars.held_empty, 1);
         bars.abort_flag = 0;
         mbar_fence_init();
         fence_proxy_async_smem();
     }
-    if (warp == 1) {
+    if (warp == 2) {
         tmem_alloc_pair(&bars.tmem_base, 512);
         tmem_relinquish_pair();
+    }
+    if (threadIdx.x == 0) {
+        tma_prefetch_desc(&tmW);
+        tma_prefetch_desc(&tmQ);
     }
     tc_fence_before_sync();
     __syncthreads();
@@ -273,92 +338,159 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) q8_pair_kernel(const __grid_co
     const uint32_t tmem_base = bars.tmem_base;
     volatile int* abort_flag = &bars.abort_flag;
 
-    if (warp == 0) {
-        if (lane == 0) {
-            tma_prefetch_desc(&tmW);
-            tma_prefetch_desc(&tmQ);
-            int s = 0;
-            uint32_t ph = 0;
-            bool ok = true;
-            for (int u = worker; u < units && ok; u += nworkers) {
-                int m0, n0;
-                pair_tile(p, u, m0, n0);
-                n0 += (int)rank * BM;
-                m0 += (int)rank * half;
-                for (int kb = 0; kb < p.kb_total; kb += KPS, s = (s + 1 == PAIR_STAGES ? 0 : s + 1), ph ^= (s == 0)) {
-                    if (!mbar_wait(&bars.empty[s], ph ^ 1, abort_flag)) { ok = false; break; }
-                    const int g = min(KPS, p.kb_total - kb);
-                    uint8_t* st = smem + s * st_bytes;
-                    const uint32_t full = mapa_shared(&bars.full[s], 0);
-                    if (rank == 0) mbar_expect_tx(&bars.full[s], (uint32_t)(2 * g * (A_BYTES + b_bytes)));
-                    for (int j = 0; j < g; ++j) {
-                        tma_load_2d_pair(st + j * A_BYTES, &tmW, full, (kb + j) * BK, n0);
-                        tma_load_2d_pair(st + KPS * A_BYTES + j * b_bytes, &tmQ, full, (kb + j) * BK, m0);
-                    }
+    if (warp == 0 || warp == 1) {
+        // Producer `warp` brings the first or second k-block of every stage (a copy costs its issuing thread 100 to 200 cycles: one thread
+        // for all of them was half as long as the products they feed).
+        const int j = warp;
+        const bool lead = elect_one();
+        int s = 0, held_n0 = -1, loads = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (Units<HELD> it(p, worker, workers); it.more() && ok; it.next()) {
+            int m0, n0;
+            it.tile(p, n0, m0);
+            if (HELD && n0 != held_n0) {
+                // other weights: once the products with the ones held so far have been made
+                if (loads > 0) {
+                    ok = mbar_wait(&bars.held_empty, (loads - 1) & 1, abort_flag);
+                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                 }
+                if (lead) {
+                    const uint32_t full = mapa_shared(&bars.held_full, 0);
+                    if (rank == 0) mbar_expect_tx(&bars.held_full, (uint32_t)(2 * ((p.kb_total + 1 - j) / 2) * A_BYTES));
+                    for (int kb = j; kb < p.kb_total; kb += 2) tma_load_2d_pair(smem + kb * A_BYTES, &tmW, full, kb * BK, n0 + (int)rank * BM);
+                }
+                __syncwarp();
+                held_n0 = n0;
+                ++loads;
             }
-            // the CTA may not retire while commits can still arrive on `empty`
-            for (int i = 0; i < PAIR_STAGES && ok; ++i, s = (s + 1 == PAIR_STAGES ? 0 : s + 1), ph ^= (s == 0))
-                if (!mbar_wait(&bars.empty[s], ph ^ 1, abort_flag)) ok = false;
-        }
-    } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
-            const uint32_t idesc = umma_idesc_s8_s32(2 * BM, p.bn);
-            const uint64_t ad0 = umma_smem_desc_sw128(smem_u32(smem), 16, 1024), bd0 = umma_smem_desc_sw128(smem_u32(smem + KPS * A_BYTES), 16, 1024);
-            int s = 0, it = 0;
-            uint32_t ph = 0;
-            bool ok = true;
-            for (int u = worker; u < units && ok; u += nworkers, ++it) {
-                const int buf = it & 1;
-                if (!mbar_wait(&bars.acc_empty[buf], ((it >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
-                tc_fence_after_sync();
-                uint32_t acc = 0;
-                for (int kb = 0; kb < p.kb_total; kb += KPS) {
-                    if (!mbar_wait(&bars.full[s], ph, abort_flag)) { ok = false; break; }
-                    tc_fence_after_sync();
-                    const int g = min(KPS, p.kb_total - kb);
-                    for (int j = 0; j < g; ++j) {
-                        uint64_t ad = ad0 + (uint32_t)((s * st_bytes + j * A_BYTES) >> 4), bd = bd0 + (uint32_t)((s * st_bytes + j * b_bytes) >> 4);
-                        const int n = instructions(p, kb + j);
-                        if (n == BK / UK) {
-#pragma unroll
-                            for (int k = 0; k < BK / UK; ++k, ad += 2, bd += 2, acc = 1) umma_s8_ss_pair(tmem_base + buf * 256, ad, bd, idesc, acc);
-                        } else {
-                            for (int k = 0; k < n; ++k, ad += 2, bd += 2, acc = 1) umma_s8_ss_pair(tmem_base + buf * 256, ad, bd, idesc, acc);
-                        }
+            n0 += (int)rank * BM;
+            m0 += (int)rank * half;
+            for (int kb = j; kb < p.kb_total + j; kb += KPS, s = (s + 1 == PAIR_STAGES ? 0 : s + 1), ph ^= (s == 0)) {
+                ok = mbar_wait(&bars.empty[s], ph ^ 1, abort_flag);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                if (lead) {
+                    const bool some = kb < p.kb_total;   // the second half of a tile's last stage may be empty
+                    uint8_t* st = ring + s * st_bytes;
+                    const uint32_t full = mapa_shared(&bars.full[s], 0);
+                    if (rank == 0) mbar_expect_tx(&bars.full[s], some ? (uint32_t)(2 * ((HELD ? 0 : A_BYTES) + b_bytes)) : 0u);
+                    if (some) {
+                        if (!HELD) tma_load_2d_pair(st + j * A_BYTES, &tmW, full, kb * BK, n0);
+                        tma_load_2d_pair(st + b_at + j * b_bytes, &tmQ, full, kb * BK, m0);
                     }
-                    umma_commit_pair(&bars.empty[s], 3);
-                    if (++s == PAIR_STAGES) { s = 0; ph ^= 1u; }
                 }
-                if (ok) umma_commit_pair(&bars.acc_full[buf], 3);
+                __syncwarp();
+            }
+        }
+        // the CTA may not retire while commits can still arrive on its barriers
+        for (int i = 0; i < PAIR_STAGES && ok; ++i, s = (s + 1 == PAIR_STAGES ? 0 : s + 1), ph ^= (s == 0))
+            if (!mbar_wait(&bars.empty[s], ph ^ 1, abort_flag)) ok = false;
+    } else if (warp == 2) {
+        // The whole warp runs the loop and one elected lane issues: with warp-uniform descriptors an instruction costs the issuing warp 40
+        // cycles instead of 48. Whole stages are straight code; only the last stage of a tile counts its instructions.
+        if (rank == 0) {
+            const bool lead = elect_one();
+            const uint32_t idesc = umma_idesc_s8_s32(2 * BM, p.bn);
+            const uint64_t ad0 = umma_smem_desc_sw128(smem_u32(smem), 16, 1024), bd0 = umma_smem_desc_sw128(smem_u32(ring + b_at), 16, 1024);
+            const uint32_t st16 = (uint32_t)st_bytes >> 4, b16 = (uint32_t)b_bytes >> 4;
+            const int last_kb = (p.kb_total - 1) / KPS * KPS;                       // first k-block of the last stage
+            const int last_n = (p.K - last_kb * BK + UK - 1) / UK;                  // its instructions, 1 to 8
+            int s = 0, i = 0, held_n0 = -1, loads = 0;
+            uint32_t ph = 0, off = 0;
+            bool ok = true;
+            for (Units<HELD> it(p, worker, workers); it.more() && ok; it.next(), ++i) {
+                const int buf = i & 1;
+                if (HELD) {
+                    int m0, n0;
+                    it.tile(p, n0, m0);
+                    if (n0 != held_n0) {
+                        if (loads > 0 && lead) umma_commit_pair(&bars.held_empty, 3);   // behind the last product with the previous weights
+                        ok = mbar_wait(&bars.held_full, loads & 1, abort_flag);
+                        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                        held_n0 = n0;
+                        ++loads;
+                    }
+                }
+                ok = mbar_wait(&bars.acc_empty[buf], ((i >> 1) & 1) ^ 1, abort_flag);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                tc_fence_after_sync();
+                const uint32_t d = tmem_base + buf * 256;
+                for (int kb = 0; kb < p.kb_total; kb += KPS) {
+                    ok = mbar_wait(&bars.full[s], ph, abort_flag);
+                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                    tc_fence_after_sync();
+                    const uint64_t ad = ad0 + (HELD ? (uint32_t)kb * (A_BYTES >> 4) : off), bd = bd0 + off, bd1 = bd + b16;
+                    if (lead) {
+                        const int n = kb == last_kb ? last_n : 8;
+                        umma_s8_ss_pair(d, ad, bd, idesc, kb > 0);
+                        if (n == 8) {
+#pragma unroll
+                            for (int k = 1; k < 4; ++k) umma_s8_ss_pair(d, ad + 2 * k, bd + 2 * k, idesc, 1);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) umma_s8_ss_pair(d, ad + (A_BYTES >> 4) + 2 * k, bd1 + 2 * k, idesc, 1);
+                        } else {
+#pragma unroll
+                            for (int k = 1; k < 7; ++k)
+                                if (k < n) umma_s8_ss_pair(d, ad + (k >> 2) * (A_BYTES >> 4) + 2 * (k & 3), (k < 4 ? bd : bd1) + 2 * (k & 3), idesc, 1);
+                        }
+                        umma_commit_pair(&bars.empty[s], 3);
+                    }
+                    __syncwarp();
+                    if (++s == PAIR_STAGES) { s = 0; ph ^= 1u; off = 0; }
+                    else off += st16;
+                }
+                if (ok && lead) umma_commit_pair(&bars.acc_full[buf], 3);
+                __syncwarp();
             }
         }
     } else {
-        const int qd = warp & 3;
-        float* sa = s_sa[qd];
-        int it = 0;
-        for (int u = worker; u < units; u += nworkers, ++it) {
+        // Two warps per lane quarter take the 32-token chunks of a tile in turn. A tile's scales are loaded while the tile before is stored:
+        // loaded when they are needed, their latency was a third of the epilogue.
+        const int qd = warp & 3, e = warp - 3, first = (e >> 2) * 32;
+        float* sa = s_sa[e];
+        float next_sa[4], next_sw = 0.0f;
+        const auto fetch = [&](const Units<HELD>& it) {
             int m0, n0;
-            pair_tile(p, u, m0, n0);
-            const int buf = it & 1, n = n0 + (int)rank * BM + qd * 32 + lane;
-            load_scales(p, sa, m0, lane);
-            const float sw = n < p.N ? p.wscale[n] : 0.0f;
-            if (!__all_sync(0xffffffffu, mbar_wait(&bars.acc_full[buf], (it >> 1) & 1, abort_flag))) break;
+            it.tile(p, n0, m0);
+            const int n = n0 + (int)rank * BM + qd * 32 + lane;
+            next_sw = n < p.N ? p.wscale[n] : 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int c = first + 64 * k + lane;
+                next_sa[k] = c < p.bn && m0 + c < p.M ? p.scale[m0 + c] : 0.0f;
+            }
+        };
+        Units<HELD> it(p, worker, workers);
+        if (it.more()) fetch(it);
+        for (int i = 0; it.more(); ++i) {
+            int m0, n0;
+            it.tile(p, n0, m0);
+            const int buf = i & 1, n = n0 + (int)rank * BM + qd * 32 + lane;
+            const float sw = next_sw;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sa[32 * k + lane] = next_sa[k];
+            __syncwarp();
+            it.next();
+            if (it.more()) fetch(it);
+            if (!__all_sync(0xffffffffu, mbar_wait(&bars.acc_full[buf], (i >> 1) & 1, abort_flag))) break;
             tc_fence_after_sync();
             const uint32_t t0 = tmem_base + ((uint32_t)(qd * 32) << 16) + (uint32_t)(buf * 256);
-            for (int c0 = 0; c0 < p.bn && m0 + c0 < p.M; c0 += 32) {
+            const uint32_t done = mapa_shared(&bars.acc_empty[buf], 0);
+            const float* s = sa;
+            const int stop = min(p.bn, p.M - m0);
+            for (int c0 = first; c0 < stop; c0 += 64, s += 32) {
                 uint32_t r[32];
                 tmem_ld_32x32(t0 + c0, r);
                 tmem_ld_wait();
-                if (n < p.N) store_tokens<TO>(p, m0 + c0, n, r, sa + c0, sw, min(32, p.M - m0 - c0));
+                if (c0 + 64 >= stop) {   // the accumulator has been read: the next tile but one may have it while this one is stored
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster_relaxed(done);
+                }
+                if (n < p.N) store_tokens<TO, RES>(p, m0 + c0, n, r, s, sw, min(32, p.M - m0 - c0));
                 __syncwarp();
             }
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) {
-                if (rank != 0) mbar_arrive_cluster(mapa_shared(&bars.acc_empty[buf], 0));
-                else mbar_arrive(&bars.acc_empty[buf]);
-            }
+            if (first >= stop && lane == 0) mbar_arrive_cluster_relaxed(done);   // a last tile without a chunk for this warp
         }
     }
     __syncwarp();
@@ -367,7 +499,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) q8_pair_kernel(const __grid_co
     __syncthreads();
     cluster_sync_all();   // no signal of the peer may still be on its way to this CTA's barriers
     tc_fence_after_sync();
-    if (warp == 1) tmem_dealloc_pair(tmem_base, 512);
+    if (warp == 2) tmem_dealloc_pair(tmem_base, 512);
 }
 
 // ---- launch ----------------------------------------------------------------------------------------------------------------------------
@@ -396,15 +528,15 @@ int split_stages(int bn, int kb_per) {
 }
 int split_smem(int bn, int splits, int kb_per) { return split_stages(bn, kb_per) * (A_BYTES + bn * BK) + (splits > 1 ? bn * BM * 4 : 0) + 1024; }
 
+enum { Q8_SPLIT = 0, Q8_PAIR = 1, Q8_HELD = 2 };
 struct Plan {
-    bool pair;
-    int bn, splits;
+    int kind, bn, splits;
 };
 
 // Estimated cycles of every tile shape; the smallest is taken.
 Plan choose(int M, int N, int K, int sms) {
     const int kb = ceil_div(K, BK);
-    Plan best{false, 16, 1};
+    Plan best{Q8_SPLIT, 16, 1};
     double least = 1e30;
     for (int bn = 16; bn <= 256; bn *= 2) {
         if (bn > 16 && bn / 2 >= M) break;
@@ -415,28 +547,30 @@ Plan choose(int M, int N, int K, int sms) {
             const double block = std::max((A_BYTES + bn * BK) / 50.0, 4.0 * std::max(60.0, bn / 2.0));
             const double one = per * block + 10.0 * bn / s + (s > 1 ? 800 + 12.0 * bn : 0.0) + 800;
             const double t = 2500 + std::ceil(ctas / sms) * one;
-            if (t < least) { least = t; best = Plan{false, bn, s}; }
+            if (t < least) { least = t; best = Plan{Q8_SPLIT, bn, s}; }
         }
     }
-    for (int bn = 64; bn <= 256; bn += 32) {
-        const double units = (double)ceil_div(N, 2 * BM) * ceil_div(M, bn);
-        const double block = std::max((A_BYTES + bn * BK / 2) / 64.0, std::max(330.0, 2.0 * bn));
-        const double t = 3500 + std::ceil(units / (sms / 2)) * std::max(kb * block, 10.0 * bn) + 10.0 * bn;
-        if (t < least) { least = t; best = Plan{true, bn, 1}; }
-    }
+    for (int kind = Q8_PAIR; kind <= (kb <= HELD_BLOCKS ? Q8_HELD : Q8_PAIR); ++kind)
+        for (int bn = 64; bn <= (kind == Q8_HELD ? HELD_BN : 256); bn += 32) {
+            const double units = (double)ceil_div(N, 2 * BM) * ceil_div(M, bn);
+            const double block = std::max(((kind == Q8_HELD ? 0 : A_BYTES) + bn * BK / 2) / 43.0, std::max(330.0, 2.0 * bn));
+            const double t = 3500 + (kind == Q8_HELD ? kb * A_BYTES / 43.0 : 0.0) + std::ceil(units / (sms / 2)) * std::max(kb * block, 10.0 * bn) + 10.0 * bn;
+            if (t < least) { least = t; best = Plan{kind, bn, 1}; }
+        }
     return best;
 }
 
-template <typename TO> int launch(Q8Args p, const int8_t* q, int ldq, const int8_t* w, cudaStream_t st) {
+template <typename TO, bool RES> int launch(Q8Args p, const int8_t* q, int ldq, const int8_t* w, cudaStream_t st) {
     static std::atomic<unsigned long long> done{0};
     if (first_use_on_current_device(done)) {
-        if (cudaFuncSetAttribute(q8_pair_kernel<TO>, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM) != cudaSuccess) return -5;
-        if (cudaFuncSetAttribute(q8_split_kernel<TO>, cudaFuncAttributeMaxDynamicSharedMemorySize, split_smem(128, 2, MAX_STAGES)) != cudaSuccess) return -5;
+        if (cudaFuncSetAttribute(q8_pair_kernel<TO, RES, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM) != cudaSuccess) return -5;
+        if (cudaFuncSetAttribute(q8_pair_kernel<TO, RES, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, HELD_SMEM) != cudaSuccess) return -5;
+        if (cudaFuncSetAttribute(q8_split_kernel<TO, RES>, cudaFuncAttributeMaxDynamicSharedMemorySize, split_smem(128, 2, MAX_STAGES)) != cudaSuccess) return -5;
     }
     const int sms = sm_count_current_device();
     Plan plan = choose(p.M, p.N, p.K, sms);
-    if (const char* e = getenv("Q8_PLAN")) { int a, b, c; if (sscanf(e, "%d,%d,%d", &a, &b, &c) == 3) plan = Plan{a != 0, b, c}; }
-    if (getenv("Q8_SAY")) fprintf(stderr, "plan pair %d bn %d splits %d\n", plan.pair, plan.bn, plan.splits);
+    if (const char* e = getenv("Q8_PLAN")) { int a, b, c; if (sscanf(e, "%d,%d,%d", &a, &b, &c) == 3 && (a != Q8_HELD || (ceil_div(p.K, BK) <= HELD_BLOCKS && b <= HELD_BN)) && (a != Q8_SPLIT || (c - 1) * ceil_div(ceil_div(p.K, BK), c) < ceil_div(p.K, BK))) plan = Plan{a, b, c}; }
+    if (getenv("Q8_SAY")) fprintf(stderr, "plan kind %d bn %d splits %d\n", plan.kind, plan.bn, plan.splits);
     static const bool overlap = getenv("BM_NO_PDL") == nullptr;
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(NUM_THREADS);
@@ -452,16 +586,17 @@ template <typename TO> int launch(Q8Args p, const int8_t* q, int ldq, const int8
     p.bn = plan.bn;
     p.kb_total = ceil_div(p.K, BK);
     p.tiles_tok = ceil_div(p.M, plan.bn);
-    p.tiles_ch = ceil_div(p.N, plan.pair ? 2 * BM : BM);
-    if (!code_map(&tmW, w, p.K, p.N, p.K, BM) || !code_map(&tmQ, q, p.K, p.M, ldq, plan.pair ? plan.bn / 2 : plan.bn)) return -11;
+    p.tiles_ch = ceil_div(p.N, plan.kind == Q8_SPLIT ? BM : 2 * BM);
+    if (!code_map(&tmW, w, p.K, p.N, p.K, BM) || !code_map(&tmQ, q, p.K, p.M, ldq, plan.kind == Q8_SPLIT ? plan.bn : plan.bn / 2)) return -11;
     const int64_t tiles = (int64_t)p.tiles_ch * p.tiles_tok;
     cudaError_t e;
-    if (plan.pair) {
+    if (plan.kind != Q8_SPLIT) {
         if (tiles > 0x3fffffff) return -1;
         at[0].val.clusterDim.x = 2;
         cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, sms / 2)));
-        cfg.dynamicSmemBytes = PAIR_SMEM;
-        e = cudaLaunchKernelEx(&cfg, q8_pair_kernel<TO>, tmW, tmQ, p);
+        cfg.blockDim = dim3(PAIR_THREADS);
+        cfg.dynamicSmemBytes = plan.kind == Q8_HELD ? HELD_SMEM : PAIR_SMEM;
+        e = cudaLaunchKernelEx(&cfg, plan.kind == Q8_HELD ? q8_pair_kernel<TO, RES, true> : q8_pair_kernel<TO, RES, false>, tmW, tmQ, p);
     } else {
         if (tiles * plan.splits > 0x7fffffff) return -1;
         p.splits = plan.splits;
@@ -470,7 +605,7 @@ template <typename TO> int launch(Q8Args p, const int8_t* q, int ldq, const int8
         at[0].val.clusterDim.x = (unsigned)plan.splits;
         cfg.gridDim = dim3((unsigned)(tiles * plan.splits));
         cfg.dynamicSmemBytes = (size_t)split_smem(plan.bn, plan.splits, p.kb_per);
-        e = cudaLaunchKernelEx(&cfg, q8_split_kernel<TO>, tmW, tmQ, p);
+        e = cudaLaunchKernelEx(&cfg, q8_split_kernel<TO, RES>, tmW, tmQ, p);
     }
     if (e == cudaSuccess) return 0;
     cudaGetLastError();   // a launch that failed must not poison the status of later calls
@@ -485,7 +620,8 @@ int q8_matmul(int dtype, void* out, int ldo, const int8_t* q, int ldq, const flo
     Q8Args p = {};
     p.out = out; p.residual = residual; p.scale = scale; p.wscale = wscale;
     p.ldo = ldo; p.ldr = ldr; p.M = M; p.N = N; p.K = K; p.err = err;
-    return dtype ? launch<bf16>(p, q, ldq, w, st) : launch<float>(p, q, ldq, w, st);
+    if (dtype) return residual ? launch<bf16, true>(p, q, ldq, w, st) : launch<bf16, false>(p, q, ldq, w, st);
+    return residual ? launch<float, true>(p, q, ldq, w, st) : launch<float, false>(p, q, ldq, w, st);
 }
 
 }  // namespace bmb
