@@ -45,11 +45,22 @@ struct Q8Args {
     int* err;
 };
 
+__device__ __forceinline__ void store_pair(float* a, float* b, float2 v) {
+    *a = v.x;
+    *b = v.y;
+}
+__device__ __forceinline__ void store_pair(bf16* a, bf16* b, float2 v) {
+    const __nv_bfloat162 h = __float22bfloat162_rn(v);
+    *a = h.x;
+    *b = h.y;
+}
+
 // One channel (this lane's) of up to 32 consecutive tokens, accumulators r, token scales sa. The residual's values are all read before the
-// first store: out may be the residual. Straight code for whole chunks: with a bound per token the compiler made 21 instructions of each.
+// first store: out may be the residual. The epilogue's instructions are what a short reduction waits for (with K = 960 a tile's products take
+// 3840 cycles): whole chunks run without bounds, two tokens per multiplication and conversion.
 template <typename TO, bool RES> __device__ __forceinline__ void store_tokens(const Q8Args& p, int m, int n, const uint32_t (&r)[32], const float* sa, float sw, int tokens) {
-    TO* o = (TO*)p.out + (size_t)m * p.ldo + n;
-    const size_t step = p.ldo;
+    char* o = (char*)((TO*)p.out + (size_t)m * p.ldo + n);
+    const uint64_t step = (uint64_t)(uint32_t)p.ldo * sizeof(TO);
     float f[32];
     if (RES) {
         const TO* res = (const TO*)p.residual + (size_t)m * p.ldr + n;
@@ -58,14 +69,16 @@ template <typename TO, bool RES> __device__ __forceinline__ void store_tokens(co
         for (int i = 0; i < 32; ++i, res += rstep) f[i] = i < tokens ? to_f32(*res) : 0.0f;
     }
     if (tokens >= 32) {
+        const float2 sw2 = make_float2(sw, sw);
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
             const float4 s = *(const float4*)(sa + i);
-            const float t[4] = {s.x * sw, s.y * sw, s.z * sw, s.w * sw};
 #pragma unroll
-            for (int j = 0; j < 4; ++j, o += step) {
-                const float v = (float)(int)r[i + j] * t[j];
-                *o = from_f32<TO>(RES ? v + f[i + j] : v);
+            for (int j = 0; j < 4; j += 2, o += 2 * step) {
+                const float2 t = f2_mul(j ? make_float2(s.z, s.w) : make_float2(s.x, s.y), sw2);
+                float2 v = f2_mul(make_float2((float)(int)r[i + j], (float)(int)r[i + j + 1]), t);
+                if (RES) v = make_float2(v.x + f[i + j], v.y + f[i + j + 1]);
+                store_pair((TO*)o, (TO*)(o + step), v);
             }
         }
     } else {
@@ -73,7 +86,7 @@ template <typename TO, bool RES> __device__ __forceinline__ void store_tokens(co
         for (int i = 0; i < 32; ++i, o += step) {
             if (i >= tokens) break;
             const float v = (float)(int)r[i] * (sa[i] * sw);
-            *o = from_f32<TO>(RES ? v + f[i] : v);
+            *(TO*)o = from_f32<TO>(RES ? v + f[i] : v);
         }
     }
 }
