@@ -147,6 +147,11 @@ __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* tmap) {
     asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)tmap) : "memory");
 }
 
+// a tile into L2 only
+__device__ __forceinline__ void tma_prefetch_l2_2d(const CUtensorMap* tmap, int c0, int c1) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"((uint64_t)tmap), "r"(c0), "r"(c1) : "memory");
+}
+
 // ---- CTA pairs (cluster of 2, tcgen05 cta_group::2) ----------------------------
 __device__ __forceinline__ uint32_t cluster_ctarank() {
     uint32_t r;

@@ -18,7 +18,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <cstdio>
 #include <cstdlib>
 
 #include "ptx_sm100.cuh"
@@ -55,19 +54,27 @@ __device__ __forceinline__ void store_pair(bf16* a, bf16* b, float2 v) {
     *b = h.y;
 }
 
-// One channel (this lane's) of up to 32 consecutive tokens, accumulators r, token scales sa. The residual's values are all read before the
-// first store: out may be the residual. The epilogue's instructions are what a short reduction waits for (with K = 960 a tile's products take
-// 3840 cycles): whole chunks run without bounds, two tokens per multiplication and conversion.
-template <typename TO, bool RES> __device__ __forceinline__ void store_tokens(const Q8Args& p, int m, int n, const uint32_t (&r)[32], const float* sa, float sw, int tokens) {
+// The residual of one channel and up to 32 consecutive tokens, as stored (widened where it is added: a conversion here would wait for the
+// load). Always read before the first of these tokens is stored: out may be the residual.
+template <typename TO> __device__ __forceinline__ void load_residual(const Q8Args& p, int m, int n, TO (&f)[32], int tokens) {
+    const TO* res = (const TO*)p.residual + (size_t)m * p.ldr + n;
+    const size_t step = p.ldr;
+    if (tokens >= 32) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i, res += step) f[i] = *res;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i, res += step)
+            if (i < tokens) f[i] = *res;
+    }
+}
+// One channel (this lane's) of up to 32 consecutive tokens: accumulators r, residual f, token scales sa. The epilogue's instructions are what a
+// short reduction waits for (with K = 960 a tile's products take 3840 cycles): whole chunks run without bounds (with a bound per token the
+// compiler made 21 instructions of each), two tokens per multiplication and conversion.
+template <typename TO, bool RES>
+__device__ __forceinline__ void store_tokens(const Q8Args& p, int m, int n, const uint32_t (&r)[32], const TO (&f)[32], const float* sa, float sw, int tokens) {
     char* o = (char*)((TO*)p.out + (size_t)m * p.ldo + n);
     const uint64_t step = (uint64_t)(uint32_t)p.ldo * sizeof(TO);
-    float f[32];
-    if (RES) {
-        const TO* res = (const TO*)p.residual + (size_t)m * p.ldr + n;
-        const size_t rstep = p.ldr;
-#pragma unroll
-        for (int i = 0; i < 32; ++i, res += rstep) f[i] = i < tokens ? to_f32(*res) : 0.0f;
-    }
     if (tokens >= 32) {
         const float2 sw2 = make_float2(sw, sw);
 #pragma unroll
@@ -77,7 +84,7 @@ template <typename TO, bool RES> __device__ __forceinline__ void store_tokens(co
             for (int j = 0; j < 4; j += 2, o += 2 * step) {
                 const float2 t = f2_mul(j ? make_float2(s.z, s.w) : make_float2(s.x, s.y), sw2);
                 float2 v = f2_mul(make_float2((float)(int)r[i + j], (float)(int)r[i + j + 1]), t);
-                if (RES) v = make_float2(v.x + f[i + j], v.y + f[i + j + 1]);
+                if (RES) v = make_float2(v.x + to_f32(f[i + j]), v.y + to_f32(f[i + j + 1]));
                 store_pair((TO*)o, (TO*)(o + step), v);
             }
         }
@@ -86,7 +93,7 @@ template <typename TO, bool RES> __device__ __forceinline__ void store_tokens(co
         for (int i = 0; i < 32; ++i, o += step) {
             if (i >= tokens) break;
             const float v = (float)(int)r[i] * (sa[i] * sw);
-            *(TO*)o = from_f32<TO>(RES ? v + f[i] : v);
+            *(TO*)o = from_f32<TO>(RES ? v + to_f32(f[i]) : v);
         }
     }
 }
@@ -107,6 +114,41 @@ __device__ __forceinline__ void report_abort(const Q8Args& p, volatile int* abor
     if (threadIdx.x == 0 && p.err) atomicExch(p.err, 3000);
 }
 
+// ---- few tokens ------------------------------------------------------------------------------------------------------------------------
+// A warp per channel, the lanes along K: 16 codes of every row per step, four at a time in the four-way byte product. Setting up tensor
+// memory, barriers and tensor maps costs more than the whole product of one token (1 x 960 -> 1600: 3.8 us there); here a call is a round
+// or two of loads and one reduction.
+constexpr int FEW_WARPS = 8, FEW_TOKENS = 4;
+template <typename TO, bool RES, int MT>
+__global__ void __launch_bounds__(32 * FEW_WARPS) q8_few_kernel(const Q8Args p, const int8_t* __restrict__ q, int ldq, const int8_t* __restrict__ w) {
+    const int lane = threadIdx.x & 31, n = (int)blockIdx.x * FEW_WARPS + (int)(threadIdx.x >> 5), chunks = p.K >> 4;
+    const int8_t* wr = w + (size_t)min(n, p.N - 1) * p.K;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    for (int k = lane; k < chunks; k += 32) prefetch_l2(wr + 16 * k);   // while the preceding kernel still runs
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (n >= p.N) return;
+    int acc[MT] = {};
+#pragma unroll 4
+    for (int k = lane; k < chunks; k += 32) {
+        const int4 b = *(const int4*)(wr + 16 * k);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const int4 a = *(const int4*)(q + (size_t)min(m, p.M - 1) * ldq + 16 * k);
+            acc[m] = __dp4a(a.x, b.x, __dp4a(a.y, b.y, __dp4a(a.z, b.z, __dp4a(a.w, b.w, acc[m]))));
+        }
+    }
+    int mine = 0;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int total = __reduce_add_sync(0xffffffffu, acc[m]);
+        if (lane == m) mine = total;
+    }
+    if (lane < p.M) {   // M <= MT tokens
+        const float v = (float)mine * (p.scale[lane] * p.wscale[n]);
+        ((TO*)p.out)[(size_t)lane * p.ldo + n] = from_f32<TO>(RES ? v + to_f32(((const TO*)p.residual)[(size_t)lane * p.ldr + n]) : v);
+    }
+}
+
 // ---- split-K over a cluster ------------------------------------------------------------------------------------------------------------
 struct __align__(8) SplitBarriers {
     uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc;
@@ -122,7 +164,7 @@ __global__ void __launch_bounds__(NUM_THREADS) q8_split_kernel(const __grid_cons
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const int b_bytes = p.bn * BK, stage_bytes = A_BYTES + b_bytes;
     int* red = (int*)(smem + p.stages * stage_bytes);   // [bn][128]: this CTA's partial sums
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;   // uniform for the compiler, too
     const int split = p.splits > 1 ? (int)cluster_ctarank() : 0;
     const int tile = (int)blockIdx.x / p.splits;
     const int m0 = tile / p.tiles_ch * p.bn, n0 = tile % p.tiles_ch * BM;
@@ -143,47 +185,57 @@ __global__ void __launch_bounds__(NUM_THREADS) q8_split_kernel(const __grid_cons
         tmem_alloc(&bars.tmem_base, tmem_cols);
         tmem_relinquish();
     }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (threadIdx.x == 0) {
+        // Into L2 while the preceding kernel still runs: the weights (a prefetch returns nothing, so it does not matter if that kernel is the
+        // one that writes them) and the two tensor maps.
+        tma_prefetch_desc(&tmW);
+        tma_prefetch_desc(&tmQ);
+        for (int kb = kb0; kb < kb1; ++kb) tma_prefetch_l2_2d(&tmW, kb * BK, n0);
+    }
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t tmem_base = bars.tmem_base;
     volatile int* abort_flag = &bars.abort_flag;
     bool ok = true;
 
     if (warp == 0) {
-        if (lane == 0) {
-            for (int kb = kb0, i = 0; kb < kb1 && ok; ++kb, ++i) {
-                const int s = i % p.stages;
-                if (i >= p.stages && !mbar_wait(&bars.empty[s], (i / p.stages - 1) & 1, abort_flag)) { ok = false; break; }
+        const bool lead = elect_one();
+        for (int kb = kb0, i = 0; kb < kb1 && ok; ++kb, ++i) {
+            const int s = i % p.stages;
+            if (i >= p.stages) ok = __all_sync(0xffffffffu, mbar_wait(&bars.empty[s], (i / p.stages - 1) & 1, abort_flag));
+            if (ok && lead) {
                 uint8_t* st = smem + s * stage_bytes;
                 mbar_expect_tx(&bars.full[s], (uint32_t)stage_bytes);
                 tma_load_2d(st, &tmW, &bars.full[s], kb * BK, n0);
                 tma_load_2d(st + A_BYTES, &tmQ, &bars.full[s], kb * BK, m0);
             }
-            // the CTA may not retire while commits can still arrive on `empty`
-            for (int i = max(0, kb1 - kb0 - p.stages); i < kb1 - kb0 && ok; ++i) ok = mbar_wait(&bars.empty[i % p.stages], (i / p.stages) & 1, abort_flag);
+            __syncwarp();
         }
-        __syncwarp();
+        // the CTA may not retire while commits can still arrive on `empty`
+        for (int i = max(0, kb1 - kb0 - p.stages); i < kb1 - kb0 && ok; ++i) ok = mbar_wait(&bars.empty[i % p.stages], (i / p.stages) & 1, abort_flag);
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc = umma_idesc_s8_s32(BM, p.bn);
-            uint32_t acc = 0;
-            for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
-                const int s = i % p.stages;
-                if (!mbar_wait(&bars.full[s], (i / p.stages) & 1, abort_flag)) { ok = false; break; }
+        const bool lead = elect_one();
+        const uint32_t idesc = umma_idesc_s8_s32(BM, p.bn);
+        for (int kb = kb0, i = 0; kb < kb1 && ok; ++kb, ++i) {
+            const int s = i % p.stages;
+            ok = __all_sync(0xffffffffu, mbar_wait(&bars.full[s], (i / p.stages) & 1, abort_flag));
+            if (ok && lead) {
                 tc_fence_after_sync();
                 const uint32_t at = smem_u32(smem + s * stage_bytes);
                 const uint64_t ad = umma_smem_desc_sw128(at, 16, 1024), bd = umma_smem_desc_sw128(at + A_BYTES, 16, 1024);
                 const int n = instructions(p, kb);
+                umma_s8_ss(tmem_base, ad, bd, idesc, i > 0);
 #pragma unroll
-                for (int k = 0; k < BK / UK; ++k, acc = 1)
-                    if (k < n) umma_s8_ss(tmem_base, ad + 2 * k, bd + 2 * k, idesc, acc);
+                for (int k = 1; k < BK / UK; ++k)
+                    if (k < n) umma_s8_ss(tmem_base, ad + 2 * k, bd + 2 * k, idesc, 1);
                 umma_commit(&bars.empty[s]);
             }
-            if (ok) umma_commit(&bars.acc);
+            __syncwarp();
         }
+        if (ok && lead) umma_commit(&bars.acc);
         __syncwarp();
     } else {
         const int qd = warp & 3, n = n0 + qd * 32 + lane;
@@ -196,9 +248,12 @@ __global__ void __launch_bounds__(NUM_THREADS) q8_split_kernel(const __grid_cons
             if (p.splits == 1)
                 for (int c0 = 0; c0 < p.bn && m0 + c0 < p.M; c0 += 32) {
                     uint32_t r[32];
+                    TO f[32];
+                    const int tokens = min(p.bn, p.M - m0) - c0;
+                    if (RES && n < p.N) load_residual<TO>(p, m0 + c0, n, f, tokens);
                     tmem_ld_32x32(tmem_base + ((uint32_t)(qd * 32) << 16) + c0, r);
                     tmem_ld_wait();
-                    if (n < p.N) store_tokens<TO, RES>(p, m0 + c0, n, r, sa + c0, sw, min(min(32, p.bn - c0), p.M - m0 - c0));
+                    if (n < p.N) store_tokens<TO, RES>(p, m0 + c0, n, r, f, sa + c0, sw, tokens);
                     __syncwarp();
                 }
         }
@@ -206,7 +261,10 @@ __global__ void __launch_bounds__(NUM_THREADS) q8_split_kernel(const __grid_cons
     if (p.splits > 1) {
         // Partial sums into this CTA's shared memory, then every CTA adds bn / splits of the columns over the cluster: a warp takes a token,
         // a lane four channels of it, 16 bytes from each CTA.
-        const int own = p.bn / p.splits, qd = warp & 3;
+        const int own = p.bn / p.splits, qd = warp & 3, n = n0 + 4 * lane;
+        float sw[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sw[i] = warp >= 2 && n + i < p.N ? p.wscale[n + i] : 0.0f;
         if (warp >= 2 && ok) {
             for (int c0 = 0; c0 < p.bn; c0 += 32) {
                 uint32_t r[32];
@@ -221,10 +279,15 @@ __global__ void __launch_bounds__(NUM_THREADS) q8_split_kernel(const __grid_cons
         __syncwarp();
         cluster_sync_all();
         if (warp >= 2) {
-            const int n = n0 + 4 * lane;
             for (int c = qd; c < own; c += 4) {
                 const int j = split * own + c, m = m0 + j;
                 if (m >= p.M || n >= p.N) break;
+                float f[4] = {};
+                if (RES) {
+                    const TO* res = (const TO*)p.residual + (size_t)m * p.ldr + n;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) f[i] = n + i < p.N ? to_f32(res[i]) : 0.0f;
+                }
                 const uint32_t at = smem_u32(red + j * BM + 4 * lane);
                 int4 sum = make_int4(0, 0, 0, 0);
 #pragma unroll 4
@@ -235,12 +298,11 @@ __global__ void __launch_bounds__(NUM_THREADS) q8_split_kernel(const __grid_cons
                 const int part[4] = {sum.x, sum.y, sum.z, sum.w};
                 const float sa = s_sa[qd][j];
                 TO* o = (TO*)p.out + (size_t)m * p.ldo + n;
-                const TO* res = RES ? (const TO*)p.residual + (size_t)m * p.ldr + n : nullptr;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (n + i < p.N) {
-                        const float v = (float)part[i] * (sa * p.wscale[n + i]);
-                        o[i] = from_f32<TO>(RES ? v + to_f32(res[i]) : v);
+                        const float v = (float)part[i] * (sa * sw[i]);
+                        o[i] = from_f32<TO>(RES ? v + f[i] : v);
                     }
             }
         }
@@ -256,18 +318,19 @@ __global__ void __launch_bounds__(NUM_THREADS) q8_split_kernel(const __grid_cons
 }
 
 // ---- persistent CTA pairs --------------------------------------------------------------------------------------------------------------
-// HELD = false: both operands stream through the ring, tiles of 256 channels x bn tokens in raster order.
-// HELD = true (K of at most HELD_BLOCKS k-blocks): a tile's weights stay in shared memory while the pair walks the tokens, so that a tile
-// moves half the bytes. With both operands streaming, every k-block of a 256 x 256 tile brings 32 KB to each SM for 512 cycles of products,
-// and the L2 gives an SM about 43 bytes per cycle when all of them ask: 760 cycles per k-block at any K.
+// A pair computes 256 channels x bn tokens; K streams through a shared-memory ring, the accumulators of the next tile are filled while this
+// one is stored. HELD (K of at most HELD_BLOCKS k-blocks): a tile's weights stay in shared memory while the pair walks the tokens, which halves
+// the bytes of a tile. With both operands streaming, every k-block of a 256 x 256 tile brings 32 KB to each SM for 512 cycles of products; the
+// L2 gives an SM 45 to 60 bytes per cycle when all of them ask, the output's bytes included (32768 x 960 -> 5120: 131 us held, 138 streamed).
+// Tokens as the A operand, their rows stored in 16-byte pieces through shared memory, was slower (145 us): the products' own operand reads and
+// the copies already fill most of the 128 bytes that an SM's shared memory moves per cycle.
 constexpr int KPS = 2;                    // k-blocks per ring stage: one wait and one commit for eight instructions
 constexpr int PAIR_STAGES = 3;
 constexpr int HELD_BLOCKS = 8;
 constexpr int HELD_BN = 224;              // widest token tile whose ring fits beside 128 KB of weights
-constexpr int EPI_WARPS = 8;              // two per lane quarter, taking 32-token chunks in turn
+constexpr int EPI_WARPS = 8;              // two per lane quarter, taking 32-column chunks in turn
 constexpr int PAIR_THREADS = 96 + 32 * EPI_WARPS;   // warps 0 and 1 copy, warp 2 issues the products
-constexpr int PAIR_SMEM = PAIR_STAGES * KPS * 2 * A_BYTES + 1024;
-constexpr int HELD_SMEM = HELD_BLOCKS * A_BYTES + PAIR_STAGES * KPS * (HELD_BN / 2) * BK + 1024;
+constexpr int pair_smem(bool held) { return (held ? HELD_BLOCKS * A_BYTES + PAIR_STAGES * KPS * (HELD_BN / 2) * BK : PAIR_STAGES * KPS * 2 * A_BYTES) + 1024; }
 
 struct __align__(8) PairBarriers {
     uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], acc_full[2], acc_empty[2], held_full, held_empty;
@@ -290,17 +353,18 @@ template <bool HELD> struct Units {
     __device__ __forceinline__ void next() { u += step; }
     // first channel and token of the unit
     __device__ __forceinline__ void tile(const Q8Args& p, int& n0, int& m0) const {
+        int tok, ch;
         if (HELD) {
-            const int c = u / p.tiles_tok;
-            n0 = c * 2 * BM;
-            m0 = (u - c * p.tiles_tok) * p.bn;
-            return;
+            ch = u / p.tiles_tok;
+            tok = u - ch * p.tiles_tok;
+        } else {
+            const int per_group = RASTER * p.tiles_tok;
+            const int g = u / per_group, idx = u - g * per_group, w = min(RASTER, p.tiles_ch - g * RASTER);
+            tok = idx / w;
+            ch = g * RASTER + idx - tok * w;
         }
-        const int per_group = RASTER * p.tiles_tok;
-        const int g = u / per_group, idx = u - g * per_group, w = min(RASTER, p.tiles_ch - g * RASTER);
-        const int t = idx / w;
-        m0 = t * p.bn;
-        n0 = (g * RASTER + idx - t * w) * 2 * BM;
+        n0 = ch * 2 * BM;
+        m0 = tok * p.bn;
     }
 };
 
@@ -356,13 +420,13 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) q8_pair_kernel(const __grid_c
         // for all of them was half as long as the products they feed).
         const int j = warp;
         const bool lead = elect_one();
-        int s = 0, held_n0 = -1, loads = 0;
+        int s = 0, held = -1, loads = 0;
         uint32_t ph = 0;
         bool ok = true;
         for (Units<HELD> it(p, worker, workers); it.more() && ok; it.next()) {
             int m0, n0;
             it.tile(p, n0, m0);
-            if (HELD && n0 != held_n0) {
+            if (HELD && n0 != held) {
                 // other weights: once the products with the ones held so far have been made
                 if (loads > 0) {
                     ok = mbar_wait(&bars.held_empty, (loads - 1) & 1, abort_flag);
@@ -374,7 +438,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) q8_pair_kernel(const __grid_c
                     for (int kb = j; kb < p.kb_total; kb += 2) tma_load_2d_pair(smem + kb * A_BYTES, &tmW, full, kb * BK, n0 + (int)rank * BM);
                 }
                 __syncwarp();
-                held_n0 = n0;
+                held = n0;
                 ++loads;
             }
             n0 += (int)rank * BM;
@@ -408,7 +472,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) q8_pair_kernel(const __grid_c
             const uint32_t st16 = (uint32_t)st_bytes >> 4, b16 = (uint32_t)b_bytes >> 4;
             const int last_kb = (p.kb_total - 1) / KPS * KPS;                       // first k-block of the last stage
             const int last_n = (p.K - last_kb * BK + UK - 1) / UK;                  // its instructions, 1 to 8
-            int s = 0, i = 0, held_n0 = -1, loads = 0;
+            int s = 0, i = 0, held = -1, loads = 0;
             uint32_t ph = 0, off = 0;
             bool ok = true;
             for (Units<HELD> it(p, worker, workers); it.more() && ok; it.next(), ++i) {
@@ -416,11 +480,11 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) q8_pair_kernel(const __grid_c
                 if (HELD) {
                     int m0, n0;
                     it.tile(p, n0, m0);
-                    if (n0 != held_n0) {
+                    if (n0 != held) {
                         if (loads > 0 && lead) umma_commit_pair(&bars.held_empty, 3);   // behind the last product with the previous weights
                         ok = mbar_wait(&bars.held_full, loads & 1, abort_flag);
                         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-                        held_n0 = n0;
+                        held = n0;
                         ++loads;
                     }
                 }
@@ -457,8 +521,8 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) q8_pair_kernel(const __grid_c
             }
         }
     } else {
-        // Two warps per lane quarter take the 32-token chunks of a tile in turn. A tile's scales are loaded while the tile before is stored:
-        // loaded when they are needed, their latency was a third of the epilogue.
+        // Two warps per lane quarter take the 32-token chunks of a tile in turn. A tile's scales are loaded while the tile before is stored, a
+        // chunk's residual while the chunk before is: loaded when they are needed, their latency was a third of the epilogue and more.
         const int qd = warp & 3, e = warp - 3, first = (e >> 2) * 32;
         float* sa = s_sa[e];
         float next_sa[4], next_sw = 0.0f;
@@ -485,12 +549,14 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) q8_pair_kernel(const __grid_c
             __syncwarp();
             it.next();
             if (it.more()) fetch(it);
-            if (!__all_sync(0xffffffffu, mbar_wait(&bars.acc_full[buf], (i >> 1) & 1, abort_flag))) break;
-            tc_fence_after_sync();
             const uint32_t t0 = tmem_base + ((uint32_t)(qd * 32) << 16) + (uint32_t)(buf * 256);
             const uint32_t done = mapa_shared(&bars.acc_empty[buf], 0);
             const float* s = sa;
             const int stop = min(p.bn, p.M - m0);
+            TO res[32];
+            if (RES && n < p.N) load_residual<TO>(p, m0 + first, n, res, stop - first);
+            if (!__all_sync(0xffffffffu, mbar_wait(&bars.acc_full[buf], (i >> 1) & 1, abort_flag))) break;
+            tc_fence_after_sync();
             for (int c0 = first; c0 < stop; c0 += 64, s += 32) {
                 uint32_t r[32];
                 tmem_ld_32x32(t0 + c0, r);
@@ -500,7 +566,15 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) q8_pair_kernel(const __grid_c
                     __syncwarp();
                     if (lane == 0) mbar_arrive_cluster_relaxed(done);
                 }
-                if (n < p.N) store_tokens<TO, RES>(p, m0 + c0, n, r, s, sw, min(32, p.M - m0 - c0));
+                if (n < p.N) {
+                    TO f[32];
+                    if (RES) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) f[j] = res[j];
+                        load_residual<TO>(p, m0 + c0 + 64, n, res, stop - c0 - 64);
+                    }
+                    store_tokens<TO, RES>(p, m0 + c0, n, r, f, s, sw, stop - c0);
+                }
                 __syncwarp();
             }
             if (first >= stop && lane == 0) mbar_arrive_cluster_relaxed(done);   // a last tile without a chunk for this warp
@@ -541,49 +615,56 @@ int split_stages(int bn, int kb_per) {
 }
 int split_smem(int bn, int splits, int kb_per) { return split_stages(bn, kb_per) * (A_BYTES + bn * BK) + (splits > 1 ? bn * BM * 4 : 0) + 1024; }
 
-enum { Q8_SPLIT = 0, Q8_PAIR = 1, Q8_HELD = 2 };
+enum { Q8_PAIR, Q8_HELD, Q8_SPLIT, Q8_FEW };
 struct Plan {
     int kind, bn, splits;
 };
 
-// Estimated cycles of every tile shape; the smallest is taken.
-Plan choose(int M, int N, int K, int sms) {
+// The estimated time, in microseconds, of every kernel and tile that can take the product; the smallest is taken. The constants were fitted to
+// 663 products (1 to 32768 tokens, K 128 to 11008, 576 to 14336 channels, both types, with and without a residual) that were timed with every
+// plan: the plan taken is 1.3 % slower than the best one in the mean and up to 31 % (K = 128 with a residual). What the terms stand for, with
+// the bytes of a k-block at the rate that an SM gets from L2:
+//   split  2.0 of launch and set-up; 2.1 more for the two cluster barriers and the exchange; per CTA a k-block is its bytes or the 0.34 that
+//          the issuing threads need; two CTAs share an SM where their shared memory allows, and then run at half the speed each
+//   pair   2.9 (larger launch, two barriers over the pair); per tile and k-block the bytes or the products; the stores of a tile share the
+//          path to L2 with the next tile's loads. Held weights: no bytes for them, but they are loaded before the first product.
+//   few    one to four tokens: the weights' bytes, and the tokens' codes from L1 once per step of 2048 codes
+Plan choose(int M, int N, int K, bool residual, int sms) {
     const int kb = ceil_div(K, BK);
+    const double out = residual ? 1.35 : 1.0;   // bytes that cross with a stored value
     Plan best{Q8_SPLIT, 16, 1};
     double least = 1e30;
-    for (int bn = 16; bn <= 256; bn *= 2) {
-        if (bn > 16 && bn / 2 >= M) break;
-        for (int s = 1; s <= 8 && (s == 1 || bn <= 128); s *= 2) {
+    const auto offer = [&](double t, Plan plan) {
+        if (t < least) { least = t; best = plan; }
+    };
+    for (int bn = 16; bn <= 256 && (bn == 16 || bn / 2 < M); bn *= 2)
+        for (int s = 1; s <= (bn <= 128 ? 8 : 1); s *= 2) {
             const int per = ceil_div(kb, s);
-            if ((s - 1) * per >= kb) continue;
+            if ((s - 1) * per >= kb) continue;   // a CTA without a k-block
             const double ctas = (double)ceil_div(N, BM) * ceil_div(M, bn) * s;
-            const double block = std::max((A_BYTES + bn * BK) / 50.0, 4.0 * std::max(60.0, bn / 2.0));
-            const double one = per * block + 10.0 * bn / s + (s > 1 ? 800 + 12.0 * bn : 0.0) + 800;
-            const double t = 2500 + std::ceil(ctas / sms) * one;
-            if (t < least) { least = t; best = Plan{Q8_SPLIT, bn, s}; }
+            const bool two = split_smem(bn, s, per) <= 112 * 1024;
+            const double rounds = two && ctas <= 2 * sms ? std::max(1.0, ctas / sms) : std::ceil(ctas / sms);
+            offer(2.0 + (s > 1 ? 2.1 + 0.016 * bn : 0.0) + rounds * (0.2 + per * std::max((A_BYTES + bn * BK) * 1.4e-5, 0.34) + 0.015 * bn * out / s), Plan{Q8_SPLIT, bn, s});
         }
-    }
     for (int kind = Q8_PAIR; kind <= (kb <= HELD_BLOCKS ? Q8_HELD : Q8_PAIR); ++kind)
-        for (int bn = 64; bn <= (kind == Q8_HELD ? HELD_BN : 256); bn += 32) {
-            const double units = (double)ceil_div(N, 2 * BM) * ceil_div(M, bn);
-            const double block = std::max(((kind == Q8_HELD ? 0 : A_BYTES) + bn * BK / 2) / 43.0, std::max(330.0, 2.0 * bn));
-            const double t = 3500 + (kind == Q8_HELD ? kb * A_BYTES / 43.0 : 0.0) + std::ceil(units / (sms / 2)) * std::max(kb * block, 10.0 * bn) + 10.0 * bn;
-            if (t < least) { least = t; best = Plan{kind, bn, 1}; }
+        for (int bn = 64; bn <= (kind == Q8_HELD ? HELD_BN : 256) && (bn == 64 || bn / 2 < M); bn += 32) {
+            const double rounds = std::ceil((double)ceil_div(N, 2 * BM) * ceil_div(M, bn) / (sms / 2));
+            const double block = std::max({((kind == Q8_HELD ? 0 : A_BYTES) + bn / 2 * BK) * 9e-6, 1.04e-3 * bn, 0.2});
+            offer(2.9 + (kind == Q8_HELD ? 0.29 * kb : 0.0) + rounds * (kb * block + 0.0053 * bn * out) + 0.0008 * bn * out, Plan{kind, bn, 1});
         }
+    if (M <= FEW_TOKENS) offer(0.05 + 0.3 * ceil_div(K, 2048) * (1 + M) + 1.4e-7 * K * N, Plan{Q8_FEW, M, 1});
     return best;
 }
 
 template <typename TO, bool RES> int launch(Q8Args p, const int8_t* q, int ldq, const int8_t* w, cudaStream_t st) {
     static std::atomic<unsigned long long> done{0};
     if (first_use_on_current_device(done)) {
-        if (cudaFuncSetAttribute(q8_pair_kernel<TO, RES, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM) != cudaSuccess) return -5;
-        if (cudaFuncSetAttribute(q8_pair_kernel<TO, RES, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, HELD_SMEM) != cudaSuccess) return -5;
+        if (cudaFuncSetAttribute(q8_pair_kernel<TO, RES, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, pair_smem(false)) != cudaSuccess) return -5;
+        if (cudaFuncSetAttribute(q8_pair_kernel<TO, RES, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, pair_smem(true)) != cudaSuccess) return -5;
         if (cudaFuncSetAttribute(q8_split_kernel<TO, RES>, cudaFuncAttributeMaxDynamicSharedMemorySize, split_smem(128, 2, MAX_STAGES)) != cudaSuccess) return -5;
     }
     const int sms = sm_count_current_device();
-    Plan plan = choose(p.M, p.N, p.K, sms);
-    if (const char* e = getenv("Q8_PLAN")) { int a, b, c; if (sscanf(e, "%d,%d,%d", &a, &b, &c) == 3 && (a != Q8_HELD || (ceil_div(p.K, BK) <= HELD_BLOCKS && b <= HELD_BN)) && (a != Q8_SPLIT || (c - 1) * ceil_div(ceil_div(p.K, BK), c) < ceil_div(p.K, BK))) plan = Plan{a, b, c}; }
-    if (getenv("Q8_SAY")) fprintf(stderr, "plan kind %d bn %d splits %d\n", plan.kind, plan.bn, plan.splits);
+    const Plan plan = choose(p.M, p.N, p.K, RES, sms);
     static const bool overlap = getenv("BM_NO_PDL") == nullptr;
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(NUM_THREADS);
@@ -595,6 +676,17 @@ template <typename TO, bool RES> int launch(Q8Args p, const int8_t* q, int ldq, 
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = overlap ? 2 : 1;
+    if (plan.kind == Q8_FEW) {
+        using Kernel = void (*)(Q8Args, const int8_t*, int, const int8_t*);
+        const Kernel few = p.M == 1 ? (Kernel)q8_few_kernel<TO, RES, 1> : p.M == 2 ? (Kernel)q8_few_kernel<TO, RES, 2> : (Kernel)q8_few_kernel<TO, RES, FEW_TOKENS>;
+        at[0] = at[1];
+        cfg.numAttrs = overlap ? 1 : 0;
+        cfg.blockDim = dim3(32 * FEW_WARPS);
+        cfg.gridDim = dim3((unsigned)ceil_div(p.N, FEW_WARPS));
+        if (cudaLaunchKernelEx(&cfg, few, p, q, ldq, w) == cudaSuccess) return 0;
+        cudaGetLastError();
+        return -9;
+    }
     CUtensorMap tmW, tmQ;
     p.bn = plan.bn;
     p.kb_total = ceil_div(p.K, BK);
@@ -608,7 +700,7 @@ template <typename TO, bool RES> int launch(Q8Args p, const int8_t* q, int ldq, 
         at[0].val.clusterDim.x = 2;
         cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, sms / 2)));
         cfg.blockDim = dim3(PAIR_THREADS);
-        cfg.dynamicSmemBytes = plan.kind == Q8_HELD ? HELD_SMEM : PAIR_SMEM;
+        cfg.dynamicSmemBytes = (size_t)pair_smem(plan.kind == Q8_HELD);
         e = cudaLaunchKernelEx(&cfg, plan.kind == Q8_HELD ? q8_pair_kernel<TO, RES, true> : q8_pair_kernel<TO, RES, false>, tmW, tmQ, p);
     } else {
         if (tiles * plan.splits > 0x7fffffff) return -1;
