@@ -196,6 +196,11 @@ double bmx_model_arch_field(const bm_model_t* model, const char* name) {
 #undef F
     return -1.0;
 }
+int bmx_model_set_act_quant(bm_model_t* model, int bits) {
+    if (!model || (bits != 0 && bits != 8)) return -1;
+    model->act_quant = bits;
+    return 0;
+}
 int bmx_model_set_quant(bm_model_t* model, int bits) {
     if (!model || (bits != 0 && bits != 4 && bits != 8)) return -1;
     model->quant_bits = bits;

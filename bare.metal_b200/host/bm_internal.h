@@ -32,6 +32,7 @@ struct bm_model_s {
     size_t n_parameters;
     int head_size, kv_dim, kv_mul;
     int quant_bits; /* 0 = weights as stored, 8 = Q8 layer matrices for inference sessions */
+    int act_quant;  /* 8 = inference sessions multiply 8-bit activations with 8-bit weights (bmx_model_set_act_quant) */
     float* weight_buffer;
     float *embed, *ln1w, *qw, *kw, *vw, *ow, *ln2w, *gate, *up, *down, *lnfw;
 };

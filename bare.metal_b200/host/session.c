@@ -10,6 +10,10 @@
  * reference multiplies x * ((float)q * scale) for both widths (matmul_forward_q8 / matmul_forward_q4, src/kernels/forward.metal:
  * 575-650, 830-858). On the device a Q4 matrix is the reference's block content as two arrays: two codes per byte (element 2j of a
  * row in the low, 2j+1 in the high nibble of byte j) and the scales, 0.625 bytes per weight.
+ * With 8-bit activations (bmx_model_set_act_quant) every layer product is bmc_matmul_q8: its operand leaves the kernel that makes it as codes
+ * with a scale per token (norm, SwiGLU, attention output), the weights have a scale per output channel. A branch's product is stored in bf16
+ * (half a step of 2^-8 of its size, below the 1/127 steps that the next operand is rounded to) and added to the fp32 residual stream by the
+ * next norm; the last layer's is added in fp32 by the product itself.
  * The whole step is enqueued without host synchronisation and, after the first token, replayed as a CUDA graph; the
  * position lives in device memory. bm_forward with several tokens runs the same step per token, which the reference
  * establishes as equivalent to its sequence prefill (test/prefill_test.c).
@@ -22,13 +26,14 @@
 #include "bm_internal.h"
 
 typedef struct {
-    void* w;       /* int8 q[OC][C] (Q8), uint8 [OC][C/2] (Q4, two codes per byte), or bf16 / fp32 [OC][C] */
-    float* scales; /* Q8 and Q4: [OC][C/32] */
+    void* w;       /* int8 q[OC][C] (Q8, 8-bit activations), uint8 [OC][C/2] (Q4, two codes per byte), or bf16 / fp32 [OC][C] */
+    float* scales; /* Q8 and Q4: [OC][C/32]; 8-bit activations: [OC] */
     void* wx;      /* tensor-core path only: bf16 [OC][parts * C], [w | w] or [w_hi | w_hi | w_lo] of the SAME weight values */
     int parts;
     int OC, C;
 } bm_mat_t;
 
+#define BM_W_ACT8 100 /* layer matrices of a session with 8-bit activations (a value beside BMC_W_*, never passed to the backend) */
 #define BM_TC_MIN_SEQUENCES 8 /* from this many sequences on, the products run as tensor-core GEMMs */
 
 typedef struct {
@@ -50,6 +55,10 @@ struct bm_session_s {
     int *d_pos, *d_tokens, *d_next, *d_gen;
     void* att_scratch;
     void* a_op; /* tensor-core path: bf16 split operand rows */
+    int act8;   /* 8-bit activations; the next three are their buffers */
+    int8_t* q8; /* [NB][widest operand] codes */
+    float* q8s; /* [NB] scales */
+    void* y;    /* [NB][D] bf16: a branch on its way to the residual stream */
     void* pf_buf; /* prefill scratch, grows to the largest prompt seen */
     size_t pf_bytes;
     void* head_wx;
@@ -119,9 +128,32 @@ static size_t quantize_blocks(int bits, const float* src, int8_t* q, float* scal
     return bits == 4 ? bmx_quantize_q4(src, q, scales, n) : bmx_quantize_q8(src, q, scales, n);
 }
 
+/* row blocks of one matrix as codes with a scale per row, made on the device */
+static int upload_matrix_act8(bm_session_t* s, bm_mat_t* m, const float* const* parts, const int* part_rows, int n_parts, int C) {
+    bmc_ctx_t* be = s->ctx->be;
+    m->OC = 0;
+    m->C = C;
+    for (int i = 0; i < n_parts; i++) m->OC += part_rows[i];
+    const size_t n = (size_t)m->OC * C;
+    m->w = bmc_alloc(be, n);
+    m->scales = (float*)bmc_alloc(be, (size_t)m->OC * sizeof(float));
+    float* tmp = (float*)bmc_alloc(be, n * sizeof(float));
+    int rc = m->w && m->scales && tmp ? 0 : -1;
+    size_t row = 0;
+    for (int i = 0; i < n_parts && !rc; i++) {
+        rc = bmc_upload(be, tmp + row * C, parts[i], (size_t)part_rows[i] * C * sizeof(float));
+        row += part_rows[i];
+    }
+    if (!rc) rc = bmc_quantize_rows_q8(be, BMC_F32, (int8_t*)m->w, C, m->scales, tmp, C, m->OC, C);
+    if (!rc) rc = bmc_sync(be);
+    bmc_free(be, tmp);
+    return rc;
+}
+
 /* upload `rows` (OC x C fp32, given as up to three row blocks that are concatenated) in the session's weight type */
 static int upload_matrix(bm_session_t* s, bm_mat_t* m, int wtype, const float* const* parts, const int* part_rows, int n_parts, int C) {
     bmc_ctx_t* be = s->ctx->be;
+    if (wtype == BM_W_ACT8) return upload_matrix_act8(s, m, parts, part_rows, n_parts, C);
     int OC = 0;
     for (int i = 0; i < n_parts; i++) OC += part_rows[i];
     m->OC = OC;
@@ -227,6 +259,10 @@ bm_session_t* bmx_create_session_kv(bm_context_t* ctx, bm_model_t* model, int n_
         BM_LOG_ERROR("bm_create_session: fp16 weights are not supported by this backend");
         return NULL;
     }
+    if (model->act_quant && model->quant_bits) {
+        BM_LOG_ERROR("bm_create_session: 8-bit activations and Q%d weights are alternatives", model->quant_bits);
+        return NULL;
+    }
     if ((a->dim % 32) || (a->hidden_dim % 32) || ((a->n_heads * model->head_size) % 32)) {
         BM_LOG_ERROR("bm_create_session: layer widths must be multiples of 32");
         return NULL;
@@ -241,7 +277,8 @@ bm_session_t* bmx_create_session_kv(bm_context_t* ctx, bm_model_t* model, int n_
     s->tc = s->tc_weights && n_sequences >= BM_TC_MIN_SEQUENCES;
     s->MS = max_positions > 0 ? max_positions : (a->max_seq_len > 0 ? a->max_seq_len : 2048);
     const int lowp = model->precision == BM_PRECISION_BF16;
-    s->wtype = model->quant_bits == 8 ? BMC_W_Q8 : model->quant_bits == 4 ? BMC_W_Q4 : (lowp ? BMC_W_BF16 : BMC_W_F32);
+    s->act8 = model->act_quant == 8;
+    s->wtype = s->act8 ? BM_W_ACT8 : model->quant_bits == 8 ? BMC_W_Q8 : model->quant_bits == 4 ? BMC_W_Q4 : (lowp ? BMC_W_BF16 : BMC_W_F32);
     s->head_type = lowp ? BMC_W_BF16 : BMC_W_F32;
     bmc_ctx_t* be = ctx->be;
     const int L = a->n_layers, D = a->dim, H = a->hidden_dim, V = a->vocab_size, HD = model->head_size;
@@ -298,6 +335,10 @@ bm_session_t* bmx_create_session_kv(bm_context_t* ctx, bm_model_t* model, int n_
             if (QD > cmax) cmax = QD;
             DALLOC(s->a_op, (size_t)NB * 3 * cmax * 2);
         }
+        if (s->act8) {
+            const int cmax = H > QD ? (H > D ? H : D) : (QD > D ? QD : D);
+            DALLOC(s->q8, (size_t)NB * cmax); DALLOC(s->q8s, (size_t)NB * 4); DALLOC(s->y, (size_t)NB * D * 2);
+        }
         DALLOC(s->d_pos, 16); DALLOC(s->d_tokens, (size_t)NB * 4); DALLOC(s->d_next, (size_t)NB * 4);
     }
 #undef DALLOC
@@ -329,7 +370,7 @@ void bm_destroy_session(bm_session_t* s) {
     }
     bmc_free(be, s->lnf); if ((void*)s->embed != s->head) bmc_free(be, s->embed); bmc_free(be, s->head); bmc_free(be, s->cache); bmc_free(be, s->cs); bmc_free(be, s->x); bmc_free(be, s->xn);
     bmc_free(be, s->qkv); bmc_free(be, s->att); bmc_free(be, s->x1); bmc_free(be, s->gu); bmc_free(be, s->act); bmc_free(be, s->logits);
-    bmc_free(be, s->att_scratch); bmc_free(be, s->pf_buf); bmc_free(be, s->a_op); bmc_free(be, s->head_wx); bmc_free(be, s->d_pos); bmc_free(be, s->d_tokens); bmc_free(be, s->d_next); bmc_free(be, s->d_gen);
+    bmc_free(be, s->att_scratch); bmc_free(be, s->pf_buf); bmc_free(be, s->a_op); bmc_free(be, s->q8); bmc_free(be, s->q8s); bmc_free(be, s->y); bmc_free(be, s->head_wx); bmc_free(be, s->d_pos); bmc_free(be, s->d_tokens); bmc_free(be, s->d_next); bmc_free(be, s->d_gen);
     free(s->h_logits);
     free(s);
 }
@@ -341,6 +382,28 @@ void bm_reset_session(bm_session_t* s) {
 }
 
 #define TRYS(call) do { int rc__ = (call); if (rc__) { BM_LOG_ERROR("decode step: %s failed (%d)", #call, rc__); return rc__; } } while (0)
+
+/* Rows of one layer with 8-bit activations, up to its attention and behind it. x: fp32 residual stream; y: the branch that the preceding half
+ * left (bf16, NULL in front of the first layer), added to x by the norm; q8, q8s: codes of the operand at hand. */
+static int act8_qkv(bm_session_t* s, const bm_dec_layer_t* m, float* x, const void* y, int8_t* q8, float* q8s, float* qkv, int rows) {
+    bmc_ctx_t* be = s->ctx->be;
+    const int D = s->model->arch.dim;
+    TRYS(bmc_rmsnorm_q8(be, BMC_F32, q8, D, q8s, y ? x : NULL, D, x, D, BMC_BF16, y, D, m->ln1, rows, D, 1e-5f));
+    TRYS(bmc_matmul_q8(be, BMC_F32, qkv, m->qkv.OC, q8, D, q8s, (const int8_t*)m->qkv.w, m->qkv.scales, NULL, 0, rows, D, m->qkv.OC));
+    return 0;
+}
+static int act8_out_mlp(bm_session_t* s, const bm_dec_layer_t* m, float* x, void* y, const float* att, int8_t* q8, float* q8s, void* gu, int rows, int last) {
+    bmc_ctx_t* be = s->ctx->be;
+    const int D = s->model->arch.dim, H = s->model->arch.hidden_dim, QD = m->o.C;
+    TRYS(bmc_quantize_rows_q8(be, BMC_F32, q8, QD, q8s, att, QD, rows, QD));
+    TRYS(bmc_matmul_q8(be, BMC_BF16, y, D, q8, QD, q8s, (const int8_t*)m->o.w, m->o.scales, NULL, 0, rows, QD, D));
+    TRYS(bmc_rmsnorm_q8(be, BMC_F32, q8, D, q8s, x, D, x, D, BMC_BF16, y, D, m->ln2, rows, D, 1e-5f));
+    TRYS(bmc_matmul_q8(be, BMC_BF16, gu, 2 * H, q8, D, q8s, (const int8_t*)m->gu.w, m->gu.scales, NULL, 0, rows, D, 2 * H));
+    TRYS(bmc_swiglu_q8(be, BMC_BF16, q8, H, q8s, gu, (const uint16_t*)gu + H, 2 * H, rows, H));
+    if (last) TRYS(bmc_matmul_q8(be, BMC_F32, x, D, q8, H, q8s, (const int8_t*)m->down.w, m->down.scales, x, D, rows, H, D));
+    else TRYS(bmc_matmul_q8(be, BMC_BF16, y, D, q8, H, q8s, (const int8_t*)m->down.w, m->down.scales, NULL, 0, rows, H, D));
+    return 0;
+}
 
 /* one token for every sequence: tokens are in d_tokens, the position in d_pos; leaves logits, the greedy choice in d_next,
  * and advances the device position */
@@ -355,6 +418,12 @@ static int enqueue_step(bm_session_t* s) {
     const int fused = NB < 4 && D <= 3072 && H <= 3072 && QD <= 3072;
     for (int l = 0; l < L; l++) {
         const bm_dec_layer_t* y = &s->layers[l];
+        if (s->act8) {
+            TRYS(act8_qkv(s, y, s->x, l ? s->y : NULL, s->q8, s->q8s, s->qkv, NB));
+            TRYS(bmc_decode_attention_fused(be, s->att, s->qkv, s->cache, s->kv_dtype, s->cs, s->d_pos, s->att_scratch, l, NB, MS, NH, NKV, HD, scale));
+            TRYS(act8_out_mlp(s, y, s->x, s->y, s->att, s->q8, s->q8s, s->gu, NB, l + 1 == L));
+            continue;
+        }
         if (s->tc) {
             TRYS(bmc_decode_prep(be, s->a_op, y->qkv.parts, s->x, D, 1, y->ln1, eps, s->qkv, QD + 2 * KV, NULL, 0, QD + 2 * KV, NB, D));
             TRYS(bmc_decode_gemm(be, s->qkv, QD + 2 * KV, s->a_op, y->qkv.wx, y->qkv.parts, NB, D, QD + 2 * KV));
@@ -438,9 +507,12 @@ static int prefill(bm_session_t* s, const int* tokens, int T) {
     int cmax = D > H ? D : H;
     if (QD > cmax) cmax = QD;
     /* one grow-only scratch allocation, carved into 256-byte aligned pieces */
-    size_t sizes[8] = {R * D * 4, R * D * 4, R * W * 4, R * QD * 4, R * 2 * H * 4, (size_t)NB * NH * T * 4, R * 3 * cmax * 2, R * sizeof(int)};
-    size_t offs[8], total = 0;
-    for (int i = 0; i < 8; i++) { offs[i] = total; total += (sizes[i] + 255) / 256 * 256; }
+    /* with 8-bit activations the bf16 operand rows shrink to codes, the branch (bf16) takes the place of the second stream buffer, and the
+     * operand that stays in bf16 is the classifier's, one row per sequence */
+    size_t sizes[9] = {R * D * 4, R * D * (s->act8 ? 2 : 4), R * W * 4, R * QD * 4, R * 2 * H * (s->act8 ? 2 : 4), (size_t)NB * NH * T * 4,
+                       s->act8 ? R * cmax + (size_t)NB * 3 * D * 2 : R * 3 * cmax * 2, R * sizeof(int), s->act8 ? R * 4 : 0};
+    size_t offs[9], total = 0;
+    for (int i = 0; i < 9; i++) { offs[i] = total; total += (sizes[i] + 255) / 256 * 256; }
     int rc = -1;
     if (total > s->pf_bytes) {
         bmc_sync(be);
@@ -454,17 +526,26 @@ static int prefill(bm_session_t* s, const int* tokens, int T) {
     float *gu = (float*)(base + offs[4]), *lse = (float*)(base + offs[5]);
     void* aop = base + offs[6];
     int* dtok = (int*)(base + offs[7]);
+    float* q8s = (float*)(base + offs[8]);
 #define TRYP(call) do { rc = (call); if (rc) { BM_LOG_ERROR("prefill: %s failed (%d)", #call, rc); goto done; } } while (0)
     TRYP(bmc_upload(be, dtok, tokens, R * sizeof(int)));
     TRYP(bmc_decode_embed(be, x, BMC_W_F32, s->embed, dtok, (int)R, D));
     for (int l = 0; l < L; l++) {
         const bm_dec_layer_t* y = &s->layers[l];
-        TRYP(bmc_decode_prep(be, aop, y->qkv.parts, x, D, 1, y->ln1, eps, qkv, W, NULL, 0, W, (int)R, D));
-        TRYP(bmc_decode_gemm(be, qkv, W, aop, y->qkv.wx, y->qkv.parts, (int)R, D, W));
+        if (s->act8) {
+            TRYP(act8_qkv(s, y, x, l ? (void*)x1 : NULL, (int8_t*)aop, q8s, qkv, (int)R));
+        } else {
+            TRYP(bmc_decode_prep(be, aop, y->qkv.parts, x, D, 1, y->ln1, eps, qkv, W, NULL, 0, W, (int)R, D));
+            TRYP(bmc_decode_gemm(be, qkv, W, aop, y->qkv.wx, y->qkv.parts, (int)R, D, W));
+        }
         TRYP(bmc_rope(be, BMC_F32, qkv, W, qkv + QD, W, s->cs, (int)R, T, NH, NKV, HD, 1));
         TRYP(bmc_decode_kv_scatter(be, s->cache, s->kv_dtype, qkv, W, l, NB, T, MS, QD, KV));
         if (HD == 64) TRYP(bmc_prefill_attention(be, att, QD, qkv, W, qkv + QD, qkv + QD + KV, W, NB, T, NH, NKV, HD, scale));
         else TRYP(bmc_attention_forward(be, BMC_F32, att, QD, lse, qkv, W, qkv + QD, qkv + QD + KV, W, NULL, NB, T, NH, NKV, HD, scale));
+        if (s->act8) {
+            TRYP(act8_out_mlp(s, y, x, x1, att, (int8_t*)aop, q8s, gu, (int)R, l + 1 == L));
+            continue;
+        }
         TRYP(bmc_decode_prep(be, aop, y->o.parts, att, QD, 0, NULL, 0.0f, x1, D, x, D, D, (int)R, QD));
         TRYP(bmc_decode_gemm(be, x1, D, aop, y->o.wx, y->o.parts, (int)R, QD, D));
         TRYP(bmc_decode_prep(be, aop, y->gu.parts, x1, D, 1, y->ln2, eps, gu, 2 * H, NULL, 0, 2 * H, (int)R, D));
@@ -472,7 +553,8 @@ static int prefill(bm_session_t* s, const int* tokens, int T) {
         TRYP(bmc_decode_prep(be, aop, y->down.parts, gu, 2 * H, 2, NULL, 0.0f, x, D, x1, D, D, (int)R, H));
         TRYP(bmc_decode_gemm(be, x, D, aop, y->down.wx, y->down.parts, (int)R, H, D));
     }
-    /* only the last row of each sequence feeds the classifier */
+    /* only the last row of each sequence feeds the classifier (its operand lies behind the codes where those are bytes) */
+    if (s->act8) aop = (char*)aop + R * cmax;
     TRYP(bmc_decode_prep(be, aop, s->head_parts, x + (size_t)(T - 1) * D, T * D, 1, s->lnf, eps, s->logits, V, NULL, 0, V, NB, D));
     TRYP(bmc_decode_gemm(be, s->logits, V, aop, s->head_wx, s->head_parts, NB, D, V));
     TRYP(bmc_decode_argmax(be, s->d_next, s->logits, NB, V));
@@ -592,7 +674,7 @@ size_t bmx_session_algorithmic_weight_bytes(bm_session_t* s) {
         const bm_mat_t* ms[4] = {&s->layers[l].qkv, &s->layers[l].o, &s->layers[l].gu, &s->layers[l].down};
         for (int i = 0; i < 4; i++) {
             const size_t e = (size_t)ms[i]->OC * ms[i]->C;
-            n += s->wtype == BMC_W_Q8 ? e + e / 32 * 4 : s->wtype == BMC_W_Q4 ? e / 2 + e / 32 * 4 : s->wtype == BMC_W_BF16 ? e * 2 : e * 4;
+            n += s->act8 ? e + (size_t)ms[i]->OC * 4 : s->wtype == BMC_W_Q8 ? e + e / 32 * 4 : s->wtype == BMC_W_Q4 ? e / 2 + e / 32 * 4 : s->wtype == BMC_W_BF16 ? e * 2 : e * 4;
         }
     }
     n += (size_t)s->model->arch.vocab_size * s->model->arch.dim * (s->head_type == BMC_W_BF16 ? 2 : 4);
@@ -607,7 +689,7 @@ size_t bmx_session_weight_bytes(bm_session_t* s) {
         const bm_mat_t* ms[4] = {&s->layers[l].qkv, &s->layers[l].o, &s->layers[l].gu, &s->layers[l].down};
         for (int i = 0; i < 4; i++) {
             const size_t e = (size_t)ms[i]->OC * ms[i]->C;
-            n += s->tc ? e * 2 * ms[i]->parts : s->wtype == BMC_W_Q8 ? e + e / 32 * 4 : s->wtype == BMC_W_Q4 ? e / 2 + e / 32 * 4 : s->wtype == BMC_W_BF16 ? e * 2 : e * 4;
+            n += s->act8 ? e + (size_t)ms[i]->OC * 4 : s->tc ? e * 2 * ms[i]->parts : s->wtype == BMC_W_Q8 ? e + e / 32 * 4 : s->wtype == BMC_W_Q4 ? e / 2 + e / 32 * 4 : s->wtype == BMC_W_BF16 ? e * 2 : e * 4;
         }
     }
     n += (size_t)s->model->arch.vocab_size * s->model->arch.dim * (s->tc ? 2 * s->head_parts : s->head_type == BMC_W_BF16 ? 2 : 4);

@@ -75,6 +75,12 @@ int    bmx_gemm_timing_collect(bm_context_t* ctx, double* out3);
  * Q8 / Q4 selection: the reference sets bm_model_s::quant_bits from its CLI (tools/cli.c:886); here through a call. bits = 0, 4 or 8.
  * A 4-bit session holds two codes per byte plus one fp32 scale per 32 weights (0.625 bytes per weight), the reference's Q4 block content. */
 int    bmx_model_set_quant(bm_model_t* model, int bits);
+/* 8-bit activations: bits = 8 makes the sessions created afterwards multiply 8-bit activations (a scale per token, taken where the operand of
+ * a product is made) with 8-bit weights (a scale per output channel) on the integer tensor pipe, in prefill and decode; bits = 0 (the default)
+ * goes back. Weights take one byte each (plus a scale per channel) for every batch size, where a Q8 / Q4 session of 8 or more sequences and
+ * every prefill stream two or three bf16 copies. The residual stream, attention, the KV cache and the LM head stay as they are. An
+ * alternative to bmx_model_set_quant: a session is refused for a model that has both set. The reference has no such mode. */
+int    bmx_model_set_act_quant(bm_model_t* model, int bits);
 /* The reference's Q8 block quantiser (bmt_quantize_q8, src/baremetal/quant.c:10-29,54-60) with the int8 values and the scales
  * in two arrays: q[n], scales[n/32]. Returns the number of blocks, 0 when n is not a positive multiple of 32. */
 size_t bmx_quantize_q8(const float* src, int8_t* q, float* scales, size_t n);

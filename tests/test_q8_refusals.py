@@ -73,3 +73,16 @@ def test_swiglu(lib, rc, change):
     (-1, dict(residual=A, ldr=40)), (0, dict(residual=A)), (0, dict(BT=5, OC=0, ldo=0, residual=None))])
 def test_matmul(lib, rc, change):
     assert call(lib, "matmul_q8", MATMUL, **change) == rc
+
+
+def test_session_mode(lib):
+    lib.bmx_model_set_act_quant.argtypes = [C.c_void_p, C.c_int]
+    lib.bm_create_model.restype = C.c_void_p
+    lib.bm_create_model.argtypes = [C.c_void_p, C.c_void_p]
+    lib.bm_destroy_model.argtypes = [C.c_void_p]
+    a = bmapi.make_arch("tiny")
+    m = lib.bm_create_model(None, C.byref(a))
+    assert m
+    assert [lib.bmx_model_set_act_quant(m, b) for b in (8, 0, 4, 1, -8, 16)] == [0, 0, -1, -1, -1, -1]
+    assert lib.bmx_model_set_act_quant(None, 8) == -1
+    lib.bm_destroy_model(m)
