@@ -21,6 +21,7 @@ int bm_log_verbose(void);
 struct bm_context_s {
     bm_device_t device_type;
     bmc_ctx_t* be;
+    const void* graph_session; /* the session whose step the backend's graph slot 0 holds */
 };
 
 /* Host copy of the weights: one flat fp32 buffer in the reference's model order

@@ -359,6 +359,7 @@ void bm_destroy_session(bm_session_t* s) {
     if (!s) return;
     bmc_ctx_t* be = s->ctx->be;
     bmc_sync(be);
+    if (s->ctx->graph_session == s) s->ctx->graph_session = NULL;
     if (s->layers) {
         for (int l = 0; l < s->model->arch.n_layers; l++) {
             bm_dec_layer_t* y = &s->layers[l];
@@ -476,13 +477,16 @@ static int run_step(bm_session_t* s) {
     }
     int rc;
     bmc_graph_select(be, 0);
+    /* one slot for every session of the context: another session's step may have taken it since */
+    if (s->graph_ready == 2 && s->ctx->graph_session != s) s->graph_ready = 1;
     if (s->graph_ready == 2) {
         rc = bmc_graph_launch(be);
     } else if (s->graph_ready == 1) {
+        s->ctx->graph_session = NULL;
         rc = bmc_graph_begin(be);
         if (!rc) rc = enqueue_step(s);
         if (!rc) rc = bmc_graph_end(be);
-        if (!rc) { s->graph_ready = 2; rc = bmc_graph_launch(be); }
+        if (!rc) { s->graph_ready = 2; s->ctx->graph_session = s; rc = bmc_graph_launch(be); }
         else { BM_LOG_ERROR("decode step: graph capture failed (%d), continuing without a graph", rc); s->graph_ready = -1; rc = enqueue_step(s); }
     } else {
         rc = enqueue_step(s);

@@ -154,3 +154,21 @@ def test_bytes_and_refusals(product):
     both = Session(product, "tiny", F32, quant=8)
     assert not both.sess
     both.close()
+
+
+def test_other_sessions_of_the_model_stay_as_they_are(product):
+    """A session made before the switch, and one after it is off again, give the bits of a plain model's session."""
+    toks = bmapi.lcg_tokens(11, 512, seed=4)
+    plain = Session(product, "tiny", F32, act=0)
+    want = [plain.vec(product.bm_step(plain.sess, int(t)))[0] for t in toks]
+    assert product.bmx_model_set_act_quant(plain.model, 8) == 0
+    eight = product.bm_create_session(plain.ctx, plain.model)
+    assert product.bmx_model_set_act_quant(plain.model, 0) == 0
+    again = product.bm_create_session(plain.ctx, plain.model)
+    product.bm_reset_session(plain.sess)
+    for i, t in enumerate(toks):
+        x, y = (plain.vec(product.bm_step(h, int(t)))[0] for h in (again, eight))
+        assert np.array_equal(x, want[i]) and not np.array_equal(y, want[i])
+    product.bm_destroy_session(eight)
+    product.bm_destroy_session(again)
+    plain.close()
