@@ -273,14 +273,20 @@ template <int MODE, typename TX, typename TY, int V, int NV> int launch_rows(con
     return launch(q8_row_kernel<MODE, TX, TY, V, NV, false>, (unsigned)p.rows, (unsigned)threads, 0, p, st);
 }
 
-// Threads per row. Many rows: 32 or 16 values a thread (whichever leaves fewer of the row's threads idle; loads in flight are what counts).
-// Few rows: as many threads as there are vectors, so that a row costs one load's latency and two reductions.
+// Threads per row. Many rows: 32 or 16 values a thread, whichever leaves fewer of the row's threads idle (loads in flight are what counts:
+// 32768 x 960 fp32 with a warp per row 23.5 us, with 16 or 8 values a thread 34); SwiGLU, which loads two vectors for each value, two accesses
+// (32768 x 2560 bf16 60 to 65 us, four accesses 64 to 68, one 79); bf16 rows of 1024 to 2048 columns 64 values, a warp per row (16384 x 1536
+// 13.7 us against 17.7). Few rows: as many threads as there are vectors, so that a row costs one load's latency and two reductions.
 template <int MODE, typename TX, typename TY, int V> int launch_vec(const RowArgs& p, cudaStream_t st) {
     const int vecs = (p.C + V - 1) / V;
-    constexpr int MOST = V == 1 ? 16 : 32 / V;   // accesses per thread (single elements: 16, or a block could not have 512 threads)
+    constexpr bool LONG = MODE == Q8_ROWS && V == 8;
+    constexpr int MOST = V == 1 ? 16 : LONG ? 8 : 32 / V;   // accesses per thread (single elements: 16, or a block could not have 512 threads)
     const auto threads_for = [&](int n) { return ((vecs + n - 1) / n + 31) / 32 * 32; };
-    int nv = MOST;
-    if (threads_for(nv / 2) <= 512 && threads_for(nv / 2) * (nv / 2) < threads_for(nv) * nv) nv /= 2;
+    const bool one_warp = LONG && vecs > 128 && vecs <= 256;
+    int nv = LONG && !one_warp ? MOST / 2 : MOST;
+    if (MODE == Q8_SWIGLU && V > 1) nv = 2;
+    while (threads_for(nv) > 512) nv *= 2;
+    if (!one_warp && threads_for(nv / 2) <= 512 && threads_for(nv / 2) * (nv / 2) < threads_for(nv) * nv) nv /= 2;
     while (nv > 1 && threads_for(nv / 2) <= 512 && (long)p.rows * threads_for(nv) < 148L * 512) nv /= 2;
     const int threads = threads_for(nv);
     if constexpr (MOST >= 16) {
