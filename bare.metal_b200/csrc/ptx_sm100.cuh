@@ -122,6 +122,22 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
     }
 }
 
+// The same for a barrier that other CTAs of the cluster arrive on: what they wrote before (to this CTA's shared memory) is visible behind it.
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    if (!mbar_wait(bar, parity, abort_flag)) return false;
+    uint32_t done;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t"
+        "}\n"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+
 // ---- proxy / tcgen05 fences -------------------------------------------------
 __device__ __forceinline__ void fence_proxy_async_smem() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -167,19 +183,11 @@ __device__ __forceinline__ uint32_t mapa_shared(const void* p, uint32_t rank) {
 __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// 16 bytes of shared memory of CTA `rank` of the cluster, at the address `own_addr` has in this CTA
-__device__ __forceinline__ int4 ld_cluster_v4(uint32_t own_addr, uint32_t rank) {
-    int4 v;
-    asm volatile(
-        "{\n\t"
-        ".reg .b32 a;\n\t"
-        "mapa.shared::cluster.u32 a, %4, %5;\n\t"
-        "ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [a];\n\t"
-        "}\n"
-        : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-        : "r"(own_addr), "r"(rank)
-        : "memory");
-    return v;
+// the two halves of it: every thread of every CTA of the cluster arrives once and waits once
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void st_cluster_u32(uint32_t cluster_addr, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
 }
 // arrive on an mbarrier of another CTA of the cluster (address from mapa_shared)
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {

@@ -107,10 +107,10 @@ __device__ __forceinline__ void load_scales(const Q8Args& p, float* sa, int m0, 
 __device__ __forceinline__ int instructions(const Q8Args& p, int kb) { return min(BK / UK, (p.K - kb * BK + UK - 1) / UK); }
 
 // a wait ran out somewhere in this CTA: let copies and products in flight land before their memory is given back, and say so
-__device__ __forceinline__ void report_abort(const Q8Args& p, volatile int* abort_flag) {
+__device__ __forceinline__ void report_abort(const Q8Args& p, volatile int* abort_flag, uint64_t grace_ns) {
     if (!*abort_flag) return;
     const uint64_t t0 = global_timer_ns();
-    while (global_timer_ns() - t0 < 2000000ull) __nanosleep(1000);
+    while (global_timer_ns() - t0 < grace_ns) __nanosleep(1000);
     if (threadIdx.x == 0 && p.err) atomicExch(p.err, 3000);
 }
 
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) q8_few_kernel(const Q8Args p, 
 
 // ---- split-K over a cluster ------------------------------------------------------------------------------------------------------------
 struct __align__(8) SplitBarriers {
-    uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc;
+    uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc, sums;
     uint32_t tmem_base;
     int abort_flag;
 };
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(NUM_THREADS) q8_split_kernel(const __grid_cons
     __shared__ __align__(16) float s_sa[4][256];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const int b_bytes = p.bn * BK, stage_bytes = A_BYTES + b_bytes;
-    int* red = (int*)(smem + p.stages * stage_bytes);   // [bn][128]: this CTA's partial sums
+    int* red = (int*)(smem + p.stages * stage_bytes);   // [splits][bn / splits][128]: every CTA's partial sums of this CTA's tokens
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;   // uniform for the compiler, too
     const int split = p.splits > 1 ? (int)cluster_ctarank() : 0;
     const int tile = (int)blockIdx.x / p.splits;
@@ -177,6 +177,7 @@ __global__ void __launch_bounds__(NUM_THREADS) q8_split_kernel(const __grid_cons
             mbar_init(&bars.empty[s], 1);
         }
         mbar_init(&bars.acc, 1);
+        mbar_init(&bars.sums, 4 * p.splits);   // the epilogue warps of every CTA of the cluster
         bars.abort_flag = 0;
         mbar_fence_init();
         fence_proxy_async_smem();
@@ -196,6 +197,7 @@ __global__ void __launch_bounds__(NUM_THREADS) q8_split_kernel(const __grid_cons
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
+    if (p.splits > 1) cluster_arrive();   // "this CTA runs and its barriers exist": waited for before the first store to a peer
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t tmem_base = bars.tmem_base;
     volatile int* abort_flag = &bars.abort_flag;
@@ -259,58 +261,55 @@ __global__ void __launch_bounds__(NUM_THREADS) q8_split_kernel(const __grid_cons
         }
     }
     if (p.splits > 1) {
-        // Partial sums into this CTA's shared memory, then every CTA adds bn / splits of the columns over the cluster: a warp takes a token,
-        // a lane four channels of it, 16 bytes from each CTA.
-        const int own = p.bn / p.splits, qd = warp & 3, n = n0 + 4 * lane;
+        // Every CTA finishes bn / splits of the tokens: it sends the other tokens' partial sums to their owners' shared memory, signals there,
+        // waits for its own and adds them, a warp per token, four channels a lane.
+        const int own = p.bn / p.splits, log_own = 31 - __clz(own), qd = warp & 3, n = n0 + 4 * lane;
         float sw[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) sw[i] = warp >= 2 && n + i < p.N ? p.wscale[n + i] : 0.0f;
+        __syncwarp();   // the barrier instruction wants whole warps
+        cluster_wait();
         if (warp >= 2 && ok) {
             for (int c0 = 0; c0 < p.bn; c0 += 32) {
                 uint32_t r[32];
                 tmem_ld_32x32(tmem_base + ((uint32_t)(qd * 32) << 16) + c0, r);
                 tmem_ld_wait();
-                int* to = red + c0 * BM + qd * 32 + lane;
+                const int* to = red + split * own * BM + qd * 32 + lane;
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
-                    if (i < 16 || p.bn > 16) to[i * BM] = (int)r[i];
+                    if (i < 16 || p.bn > 16) st_cluster_u32(mapa_shared(to + ((c0 + i) & (own - 1)) * BM, (uint32_t)(c0 + i) >> log_own), r[i]);
             }
-        }
-        __syncwarp();
-        cluster_sync_all();
-        if (warp >= 2) {
-            for (int c = qd; c < own; c += 4) {
+            __syncwarp();
+            if (lane < p.splits) mbar_arrive_cluster(mapa_shared(&bars.sums, (uint32_t)lane));
+            ok = __all_sync(0xffffffffu, mbar_wait_cluster(&bars.sums, 0, abort_flag));
+            for (int c = qd; c < own && ok; c += 4) {
                 const int j = split * own + c, m = m0 + j;
                 if (m >= p.M || n >= p.N) break;
-                float f[4] = {};
+                TO f[4];
                 if (RES) {
                     const TO* res = (const TO*)p.residual + (size_t)m * p.ldr + n;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) f[i] = n + i < p.N ? to_f32(res[i]) : 0.0f;
+                    for (int i = 0; i < 4; ++i)
+                        if (n + i < p.N) f[i] = res[i];
                 }
-                const uint32_t at = smem_u32(red + j * BM + 4 * lane);
-                int4 sum = make_int4(0, 0, 0, 0);
-#pragma unroll 4
+                int sum[4] = {};
                 for (int s = 0; s < p.splits; ++s) {
-                    const int4 v = ld_cluster_v4(at, (uint32_t)s);
-                    sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+                    const int4 v = *(const int4*)(red + (s * own + c) * BM + 4 * lane);
+                    sum[0] += v.x; sum[1] += v.y; sum[2] += v.z; sum[3] += v.w;
                 }
-                const int part[4] = {sum.x, sum.y, sum.z, sum.w};
                 const float sa = s_sa[qd][j];
                 TO* o = (TO*)p.out + (size_t)m * p.ldo + n;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (n + i < p.N) {
-                        const float v = (float)part[i] * (sa * sw[i]);
-                        o[i] = from_f32<TO>(RES ? v + f[i] : v);
+                        const float v = (float)sum[i] * (sa * sw[i]);
+                        o[i] = from_f32<TO>(RES ? v + to_f32(f[i]) : v);
                     }
             }
         }
-        __syncwarp();
-        cluster_sync_all();   // nobody leaves while its shared memory is still read
     }
     __syncwarp();
-    report_abort(p, abort_flag);
+    report_abort(p, abort_flag, p.splits > 1 ? 2500000000ull : 2000000ull);   // a peer may still write here until its own wait has run out, too
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
@@ -581,7 +580,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) q8_pair_kernel(const __grid_c
         }
     }
     __syncwarp();
-    report_abort(p, abort_flag);
+    report_abort(p, abort_flag, 2000000ull);
     tc_fence_before_sync();
     __syncthreads();
     cluster_sync_all();   // no signal of the peer may still be on its way to this CTA's barriers
