@@ -177,9 +177,10 @@ __global__ void __launch_bounds__(NUM_THREADS) q8_split_kernel(const __grid_cons
             mbar_init(&bars.empty[s], 1);
         }
         mbar_init(&bars.acc, 1);
-        mbar_init(&bars.sums, 4 * p.splits);   // the epilogue warps of every CTA of the cluster
+        mbar_init(&bars.sums, 1);
         bars.abort_flag = 0;
         mbar_fence_init();
+        if (p.splits > 1) mbar_expect_tx(&bars.sums, (uint32_t)(p.bn * BM * 4));   // this CTA's tokens from every CTA of the cluster
         fence_proxy_async_smem();
     }
     if (warp == 1) {
@@ -202,6 +203,7 @@ __global__ void __launch_bounds__(NUM_THREADS) q8_split_kernel(const __grid_cons
     const uint32_t tmem_base = bars.tmem_base;
     volatile int* abort_flag = &bars.abort_flag;
     bool ok = true;
+    float sw4[4];
 
     if (warp == 0) {
         const bool lead = elect_one();
@@ -244,6 +246,11 @@ __global__ void __launch_bounds__(NUM_THREADS) q8_split_kernel(const __grid_cons
         float* sa = s_sa[qd];
         load_scales(p, sa, m0, lane);
         const float sw = n < p.N ? p.wscale[n] : 0.0f;
+        if (p.splits > 1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sw4[i] = n0 + 4 * lane + i < p.N ? p.wscale[n0 + 4 * lane + i] : 0.0f;
+            cluster_wait();   // here, where there is time: the products are still being made
+        }
         ok = __all_sync(0xffffffffu, mbar_wait(&bars.acc, 0, abort_flag));
         if (ok) {
             tc_fence_after_sync();
@@ -261,14 +268,11 @@ __global__ void __launch_bounds__(NUM_THREADS) q8_split_kernel(const __grid_cons
         }
     }
     if (p.splits > 1) {
-        // Every CTA finishes bn / splits of the tokens: it sends the other tokens' partial sums to their owners' shared memory, signals there,
-        // waits for its own and adds them, a warp per token, four channels a lane.
+        // Every CTA finishes bn / splits of the tokens: partial sums go to their owners' shared memory by asynchronous stores, whose bytes the
+        // owner's barrier counts; it adds them, a warp per token, four channels a lane.
         const int own = p.bn / p.splits, log_own = 31 - __clz(own), qd = warp & 3, n = n0 + 4 * lane;
-        float sw[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sw[i] = warp >= 2 && n + i < p.N ? p.wscale[n + i] : 0.0f;
         __syncwarp();   // the barrier instruction wants whole warps
-        cluster_wait();
+        if (warp < 2) cluster_wait();
         if (warp >= 2 && ok) {
             for (int c0 = 0; c0 < p.bn; c0 += 32) {
                 uint32_t r[32];
@@ -277,10 +281,12 @@ __global__ void __launch_bounds__(NUM_THREADS) q8_split_kernel(const __grid_cons
                 const int* to = red + split * own * BM + qd * 32 + lane;
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
-                    if (i < 16 || p.bn > 16) st_cluster_u32(mapa_shared(to + ((c0 + i) & (own - 1)) * BM, (uint32_t)(c0 + i) >> log_own), r[i]);
+                    if (i < 16 || p.bn > 16) {
+                        const uint32_t owner = (uint32_t)(c0 + i) >> log_own;
+                        st_async_u32(mapa_shared(to + ((c0 + i) & (own - 1)) * BM, owner), r[i], mapa_shared(&bars.sums, owner));
+                    }
             }
             __syncwarp();
-            if (lane < p.splits) mbar_arrive_cluster(mapa_shared(&bars.sums, (uint32_t)lane));
             ok = __all_sync(0xffffffffu, mbar_wait_cluster(&bars.sums, 0, abort_flag));
             for (int c = qd; c < own && ok; c += 4) {
                 const int j = split * own + c, m = m0 + j;
@@ -302,7 +308,7 @@ __global__ void __launch_bounds__(NUM_THREADS) q8_split_kernel(const __grid_cons
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (n + i < p.N) {
-                        const float v = (float)sum[i] * (sa * sw[i]);
+                        const float v = (float)sum[i] * (sa * sw4[i]);
                         o[i] = from_f32<TO>(RES ? v + to_f32(f[i]) : v);
                     }
             }
