@@ -335,7 +335,12 @@ constexpr int HELD_BLOCKS = 8;
 constexpr int HELD_BN = 224;              // widest token tile whose ring fits beside 128 KB of weights
 constexpr int EPI_WARPS = 8;              // two per lane quarter, taking 32-column chunks in turn
 constexpr int PAIR_THREADS = 96 + 32 * EPI_WARPS;   // warps 0 and 1 copy, warp 2 issues the products
-constexpr int pair_smem(bool held) { return (held ? HELD_BLOCKS * A_BYTES + PAIR_STAGES * KPS * (HELD_BN / 2) * BK : PAIR_STAGES * KPS * 2 * A_BYTES) + 1024; }
+// All that a CTA may ask for, whatever the ring needs: a CTA of the split kernel must not run beside one of this kernel. Both hold tensor
+// memory while they wait for other CTAs of theirs; on two SMs (two streams) each could hold what the other's peer is still waiting to allocate.
+// CTAs of the split kernel alone never run out: a cluster's fit an SM at most 512 / columns times by their shared memory.
+constexpr int PAIR_SMEM = 222 * 1024;
+constexpr int pair_ring(bool held) { return held ? HELD_BLOCKS * A_BYTES + PAIR_STAGES * KPS * (HELD_BN / 2) * BK : PAIR_STAGES * KPS * 2 * A_BYTES; }
+static_assert(pair_ring(false) + 1024 <= PAIR_SMEM && pair_ring(true) + 1024 <= PAIR_SMEM, "shared memory budget");
 
 struct __align__(8) PairBarriers {
     uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], acc_full[2], acc_empty[2], held_full, held_empty;
@@ -627,16 +632,15 @@ struct Plan {
 
 // The estimated time, in microseconds, of every kernel and tile that can take the product; the smallest is taken. The constants were fitted to
 // 663 products (1 to 32768 tokens, K 128 to 11008, 576 to 14336 channels, both types, with and without a residual) that were timed with every
-// plan: the plan taken is 1.3 % slower than the best one in the mean and up to 31 % (K = 128 with a residual). What the terms stand for, with
-// the bytes of a k-block at the rate that an SM gets from L2:
-//   split  2.0 of launch and set-up; 2.1 more for the two cluster barriers and the exchange; per CTA a k-block is its bytes or the 0.34 that
-//          the issuing threads need; two CTAs share an SM where their shared memory allows, and then run at half the speed each
-//   pair   2.9 (larger launch, two barriers over the pair); per tile and k-block the bytes or the products; the stores of a tile share the
-//          path to L2 with the next tile's loads. Held weights: no bytes for them, but they are loaded before the first product.
+// plan: the plan taken is 1.2 % slower than the best one in the mean and 27 % at the most (K = 128 with a residual). What the terms stand for,
+// with the bytes of a k-block at the rate that an SM gets from L2:
+//   split  2.1 of launch and set-up, more for the exchange over a cluster; per CTA a k-block is its bytes, or the 0.32 that its issuing threads
+//          need, and a token its stores; two CTAs share an SM where their shared memory allows, and then run at half the speed each
+//   pair   2.3; per tile and k-block the bytes, the products or the issuing threads; the stores of a tile share the path to L2 with the next
+//          tile's loads. Held weights: no bytes for them, but they are loaded before the first product.
 //   few    one to four tokens: the weights' bytes, and the tokens' codes from L1 once per step of 2048 codes
-Plan choose(int M, int N, int K, bool residual, int sms) {
+Plan choose(int M, int N, int K, int sms) {
     const int kb = ceil_div(K, BK);
-    const double out = residual ? 1.35 : 1.0;   // bytes that cross with a stored value
     Plan best{Q8_SPLIT, 16, 1};
     double least = 1e30;
     const auto offer = [&](double t, Plan plan) {
@@ -649,27 +653,27 @@ Plan choose(int M, int N, int K, bool residual, int sms) {
             const double ctas = (double)ceil_div(N, BM) * ceil_div(M, bn) * s;
             const bool two = split_smem(bn, s, per) <= 112 * 1024;
             const double rounds = two && ctas <= 2 * sms ? std::max(1.0, ctas / sms) : std::ceil(ctas / sms);
-            offer(2.0 + (s > 1 ? 2.1 + 0.016 * bn : 0.0) + rounds * (0.2 + per * std::max((A_BYTES + bn * BK) * 1.4e-5, 0.34) + 0.015 * bn * out / s), Plan{Q8_SPLIT, bn, s});
+            offer(2.1 + (s > 1 ? 0.16 + 0.044 * bn : 0.0) + rounds * (per * std::max((A_BYTES + bn * BK) * 1.6e-5, 0.32) + 0.0073 * bn / s), Plan{Q8_SPLIT, bn, s});
         }
     for (int kind = Q8_PAIR; kind <= (kb <= HELD_BLOCKS ? Q8_HELD : Q8_PAIR); ++kind)
         for (int bn = 64; bn <= (kind == Q8_HELD ? HELD_BN : 256) && (bn == 64 || bn / 2 < M); bn += 32) {
             const double rounds = std::ceil((double)ceil_div(N, 2 * BM) * ceil_div(M, bn) / (sms / 2));
-            const double block = std::max({((kind == Q8_HELD ? 0 : A_BYTES) + bn / 2 * BK) * 9e-6, 1.04e-3 * bn, 0.2});
-            offer(2.9 + (kind == Q8_HELD ? 0.29 * kb : 0.0) + rounds * (kb * block + 0.0053 * bn * out) + 0.0008 * bn * out, Plan{kind, bn, 1});
+            const double block = std::max({((kind == Q8_HELD ? 0 : A_BYTES) + bn / 2 * BK) * 8.1e-6, 8.8e-4 * bn, 0.21});
+            offer(2.3 + (kind == Q8_HELD ? 0.23 * kb : 0.0) + rounds * (kb * block + 0.0052 * bn), Plan{kind, bn, 1});
         }
-    if (M <= FEW_TOKENS) offer(0.05 + 0.3 * ceil_div(K, 2048) * (1 + M) + 1.4e-7 * K * N, Plan{Q8_FEW, M, 1});
+    if (M <= FEW_TOKENS) offer(0.11 + 0.41 * ceil_div(K, 2048) * (1 + M) + (1.1e-7 + 1.5e-8 * M) * K * N, Plan{Q8_FEW, M, 1});
     return best;
 }
 
 template <typename TO, bool RES> int launch(Q8Args p, const int8_t* q, int ldq, const int8_t* w, cudaStream_t st) {
     static std::atomic<unsigned long long> done{0};
     if (first_use_on_current_device(done)) {
-        if (cudaFuncSetAttribute(q8_pair_kernel<TO, RES, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, pair_smem(false)) != cudaSuccess) return -5;
-        if (cudaFuncSetAttribute(q8_pair_kernel<TO, RES, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, pair_smem(true)) != cudaSuccess) return -5;
+        if (cudaFuncSetAttribute(q8_pair_kernel<TO, RES, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM) != cudaSuccess) return -5;
+        if (cudaFuncSetAttribute(q8_pair_kernel<TO, RES, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM) != cudaSuccess) return -5;
         if (cudaFuncSetAttribute(q8_split_kernel<TO, RES>, cudaFuncAttributeMaxDynamicSharedMemorySize, split_smem(128, 2, MAX_STAGES)) != cudaSuccess) return -5;
     }
     const int sms = sm_count_current_device();
-    const Plan plan = choose(p.M, p.N, p.K, RES, sms);
+    const Plan plan = choose(p.M, p.N, p.K, sms);
     static const bool overlap = getenv("BM_NO_PDL") == nullptr;
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(NUM_THREADS);
@@ -705,7 +709,7 @@ template <typename TO, bool RES> int launch(Q8Args p, const int8_t* q, int ldq, 
         at[0].val.clusterDim.x = 2;
         cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, sms / 2)));
         cfg.blockDim = dim3(PAIR_THREADS);
-        cfg.dynamicSmemBytes = (size_t)pair_smem(plan.kind == Q8_HELD);
+        cfg.dynamicSmemBytes = PAIR_SMEM;
         e = cudaLaunchKernelEx(&cfg, plan.kind == Q8_HELD ? q8_pair_kernel<TO, RES, true> : q8_pair_kernel<TO, RES, false>, tmW, tmQ, p);
     } else {
         if (tiles * plan.splits > 0x7fffffff) return -1;
