@@ -10,6 +10,8 @@ that is off by at most 127 (2 t + 4 u), so |code * scale - v| <= (1/2 + 127 (2 t
   swiglu the exponential's argument is off by 2 |g| u absolutely and the exponential by 4 u; four more roundings: t = (2 |g| + 12) u
   product: conversion of the sum, product of the scales, their product: 3 u of the product; u of the sum with the residual; the store."""
 import ctypes as C
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -440,3 +442,40 @@ def test_side_stream(be):
     assert ticket >= 0 and be.lib.bmc_side_wait(ctx, ticket) == 0
     for m, w in zip((a, b), want):
         assert np.array_equal(be.get(m.out, (m.rows, m.D)), w)
+
+
+FIRST_USE_IN_A_CAPTURE = """
+import ctypes as C, sys
+import numpy as np
+sys.path.insert(0, "bare.metal_b200"); sys.path.insert(0, "tests")
+import bmapi, bmcapi, test_gpu_q8_ops as t
+be = bmcapi.Backend(bmapi.load_product())
+rng = np.random.default_rng(1)
+ctx = C.c_void_p(be.ctx)
+todo = []
+for M, K, N in ((1, 960, 200), (24, 2560, 130), (600, 960, 1600), (5000, 2048, 1600)):
+    q, w = rng.integers(-128, 128, (M, K)).astype(np.int8), rng.integers(-128, 128, (N, K)).astype(np.int8)
+    dq, dw, ds, dn, out = t.put_bytes(be, q), t.put_bytes(be, w), be.put(np.full(M, 0.5, np.float32)), be.put(np.full(N, 0.25, np.float32)), be.alloc(M * N * 4)
+    todo.append((M, K, N, q, w, dq, dw, ds, dn, out))
+x = rng.standard_normal((40, 960)).astype(np.float32)
+dx, cq, cs = be.put(x), be.alloc(40 * 960), be.alloc(160)
+assert be.lib.bmc_graph_begin(ctx) == 0
+for M, K, N, q, w, dq, dw, ds, dn, out in todo:
+    assert be.lib.bmc_matmul_q8(be.ctx, 0, out, N, dq, K, ds, dw, dn, None, 0, M, K, N) == 0
+assert be.lib.bmc_quantize_rows_q8(be.ctx, 0, cq, 960, cs, dx, 960, 40, 960) == 0
+assert be.lib.bmc_graph_end(ctx) == 0
+for _ in range(2):
+    assert be.lib.bmc_graph_launch(ctx) == 0
+assert be.lib.bmc_sync(be.ctx) == 0
+for M, K, N, q, w, dq, dw, ds, dn, out in todo:
+    got = be.get(out, (M, N))
+    want = (q.astype(np.float64) @ w.astype(np.float64).T) * 0.125
+    assert np.all(np.abs(got - want) <= 2.0 ** -24 * np.abs(want)), (M, K, N)
+t.check_codes(be.get(cq, (40, 960), np_dtype=np.int8), be.get(cs, (40,)), x.astype(np.float64), 0.0)
+"""
+
+
+def test_first_use_in_a_capture():
+    """A process whose first call of every kernel is being captured."""
+    r = subprocess.run([sys.executable, "-c", FIRST_USE_IN_A_CAPTURE], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr

@@ -41,8 +41,16 @@ class Walk:
     def rms(x, w):
         return x / np.sqrt(np.mean(x * x, axis=1, keepdims=True) + 1e-5) * w
 
-    def logits(self, tokens):
-        """[T, V] for one sequence"""
+    @staticmethod
+    def attention(q, k, v):
+        T = len(q)
+        s = np.einsum("qhd,khd->hqk", q, k) / np.sqrt(q.shape[-1])
+        s = np.where(np.tril(np.ones((T, T), bool)), s, -np.inf)
+        p = np.exp(s - s.max(-1, keepdims=True))
+        return np.einsum("hqk,khd->qhd", p / p.sum(-1, keepdims=True), v).reshape(T, -1)
+
+    def logits(self, tokens, bf16_cache_from=None):
+        """[T, V] for one sequence. From row bf16_cache_from on, keys and values are read from a bf16 cache (a prompt's own rows are not)."""
         a, w, T = self.a, self.w, len(tokens)
         HD, NH, NKV, H = a.head_dim, a.n_heads, a.n_kv_heads, a.hidden_dim
         half = lambda v: bf16_round(v.astype(np.float32)).astype(np.float64)
@@ -55,10 +63,9 @@ class Walk:
             q, k, v = np.split(qkv, [NH * HD, (NH + NKV) * HD], axis=1)
             q, k, v = rot(q.reshape(T, NH, HD)), rot(k.reshape(T, NKV, HD)), v.reshape(T, NKV, HD)
             k, v = np.repeat(k, NH // NKV, 1), np.repeat(v, NH // NKV, 1)
-            s = np.einsum("qhd,khd->hqk", q, k) / np.sqrt(HD)
-            s = np.where(np.tril(np.ones((T, T), bool)), s, -np.inf)
-            p = np.exp(s - s.max(-1, keepdims=True))
-            att = np.einsum("hqk,khd->qhd", p / p.sum(-1, keepdims=True), v).reshape(T, NH * HD)
+            att = self.attention(q, k, v)
+            if bf16_cache_from is not None:
+                att[bf16_cache_from:] = self.attention(q, half(k), half(v))[bf16_cache_from:]
             x = x + half(self.to8(att) @ self.o[l].T)
             gu = half(self.to8(self.rms(x, w["ln2w"][l])) @ self.gu[l].T)
             g, u = gu[:, :H], gu[:, H:]
@@ -68,7 +75,7 @@ class Walk:
 
 
 class Session:
-    def __init__(self, lib, name, precision, NB=1, MS=64, act=8, quant=0, seed=3):
+    def __init__(self, lib, name, precision, NB=1, MS=64, act=8, quant=0, seed=3, kv_bf16=0):
         self.lib, self.NB = lib, NB
         self.a = bmapi.make_arch(name)
         self.a.precision = precision
@@ -83,7 +90,7 @@ class Session:
         lib.bm_load_weights(self.model, path.encode())
         os.unlink(path)
         assert lib.bmx_model_set_act_quant(self.model, act) == 0 and lib.bmx_model_set_quant(self.model, quant) == 0
-        self.sess = lib.bmx_create_session_batched(self.ctx, self.model, NB, MS)
+        self.sess = lib.bmx_create_session_kv(self.ctx, self.model, NB, MS, kv_bf16)
 
     def vec(self, p):
         assert p
@@ -139,6 +146,22 @@ def test_batched_greedy(product, NB, n_prompt):
         assert near(last[b], want[-1]), b
         for i in range(n_new):
             assert want[i].max() - want[i][out[b, i]] <= 2 * FAR * np.linalg.norm(want[i]) / np.sqrt(V) * 5, (b, i)   # one logit: five times the mean error
+    s.close()
+
+
+@pytest.mark.parametrize("kv_bf16,variables", [(1, ()), (0, ("BM_NO_TC_DECODE",)), (0, ("BM_NO_GRAPH", "BM_NO_PDL"))])
+def test_other_session_settings(product, monkeypatch, kv_bf16, variables):
+    """A bf16 KV cache, no split-bf16 classifier (and so no prefill in one pass), no graph."""
+    for v in variables:
+        monkeypatch.setenv(v, "1")
+    s = Session(product, "gqa", BF16, NB=9, MS=32, kv_bf16=kv_bf16)
+    ref = Walk(s.a, s.w, BF16)
+    prompt = bmapi.lcg_tokens(9 * 10, s.a.vocab_size, seed=2).reshape(9, 10)
+    out = np.zeros((9, 4), np.int32)
+    assert s.lib.bmx_session_generate_greedy(s.sess, bmapi.as_int_ptr(np.ascontiguousarray(prompt)), 10, 4, bmapi.as_int_ptr(out)) == 0
+    last = s.vec(s.lib.bmx_session_logits(s.sess))
+    for b in range(9):
+        assert near(last[b], ref.logits(np.concatenate([prompt[b], out[b][:-1]]), 10 if kv_bf16 else None)[-1]), b
     s.close()
 
 
