@@ -123,8 +123,33 @@ template <bool WARP> __device__ __forceinline__ uint32_t row_max(uint32_t v, uin
 
 constexpr int WARP_ROWS = 4;   // rows per block where a warp has a row
 
+// V values from p[c ..] of a row that has `C` of them, those outside as 0
+template <typename T, int V> __device__ __forceinline__ void load_edge(const T* p, int c, int C, float (&f)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = c + j >= 0 && c + j < C ? to_f32(p[c + j]) : 0.0f;
+}
+// V gains from w[c ..], c = `off` (0 to 3) above a multiple of four: whole vectors, and a shift that is the same for every thread of a row
+template <int V> __device__ __forceinline__ void load_gains(const float* w, int c, int off, int C, float (&f)[V]) {
+    float t[V + 4];
+    if (c < 0 || c - off + V + 4 > C) {
+        load_edge<float, V>(w, c, C, f);
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < V / 4 + 1; ++k) {
+        const float4 x = *(const float4*)(w + c - off + 4 * k);
+        t[4 * k] = x.x; t[4 * k + 1] = x.y; t[4 * k + 2] = x.z; t[4 * k + 3] = x.w;
+    }
+#pragma unroll
+    for (int j = 0; j < V + 2; ++j) t[j] = (off & 1) ? t[j + 1] : t[j];
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = (off & 2) ? t[j + 2] : t[j];
+}
+
 // V elements per access, NV accesses per thread. WARP: a warp per row, WARP_ROWS rows per block; otherwise a block per row.
-template <int MODE, typename TX, typename TY, int V, int NV, bool WARP>
+// EDGE: rows that do not start on a vector (an odd width), but on the same element of one in every operand: the vectors lie where memory has
+// them, the first one `phase` elements before the row, and the first and last of a row are read and written element by element.
+template <int MODE, typename TX, typename TY, int V, int NV, bool WARP, bool EDGE>
 __global__ void __launch_bounds__(WARP ? 32 * WARP_ROWS : 512) q8_row_kernel(const RowArgs p) {
     __shared__ float red[32];
     __shared__ uint32_t redu[32];
@@ -135,13 +160,19 @@ __global__ void __launch_bounds__(WARP ? 32 * WARP_ROWS : 512) q8_row_kernel(con
     if (row >= p.rows) return;   // whole warps only, and only where a warp has a row
     const TX* x = (const TX*)p.x + (size_t)row * p.ldx;
     const TY* y = (const TY*)p.y + (size_t)row * p.ldy;
+    TX* sum = MODE == Q8_NORM && p.sum ? (TX*)p.sum + (size_t)row * p.lds : nullptr;
+    int8_t* q = p.q + (size_t)row * p.ldq;
     const bool has_y = MODE == Q8_SWIGLU || (MODE == Q8_NORM && p.y != nullptr);
+    const int phase = EDGE ? (int)(((uintptr_t)x / sizeof(TX)) & (V - 1)) : 0;
+    const auto column = [&](int i) { return (t + i * nt) * V - phase; };
+    const auto whole = [&](int c) { return EDGE ? c >= 0 && c + V <= p.C : c < p.C; };
+    const auto some = [&](int c) { return EDGE && c < p.C && c + V > 0; };   // of a vector that is not whole
     Pack<TX, V> px[NV];
     Pack<TY, V> py[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int c = (t + i * nt) * V;
-        if (c < p.C) {
+        const int c = column(i);
+        if (whole(c)) {
             px[i].load(x + c);
             if (has_y) py[i].load(y + c);
         }
@@ -151,16 +182,26 @@ __global__ void __launch_bounds__(WARP ? 32 * WARP_ROWS : 512) q8_row_kernel(con
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int c = (t + i * nt) * V;
-        if (c < p.C) {
-            px[i].unpack(v[i]);
+        const int c = column(i);
+        if (whole(c) || some(c)) {
+            if (whole(c)) px[i].unpack(v[i]);
+            else load_edge<TX, V>(x, c, p.C, v[i]);
             if (has_y) {
                 float f[V];
-                py[i].unpack(f);
+                if (whole(c)) py[i].unpack(f);
+                else load_edge<TY, V>(y, c, p.C, f);
 #pragma unroll
                 for (int j = 0; j < V; ++j) v[i][j] = MODE == Q8_SWIGLU ? silu(v[i][j]) * f[j] : v[i][j] + f[j];
             }
-            if (MODE == Q8_NORM && p.sum) Pack<TX, V>::store((TX*)p.sum + (size_t)row * p.lds + c, v[i]);
+            if (sum) {
+                if (whole(c)) {
+                    Pack<TX, V>::store(sum + c, v[i]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < V; ++j)
+                        if (c + j >= 0 && c + j < p.C) sum[c + j] = from_f32<TX>(v[i][j]);
+                }
+            }
         } else {
 #pragma unroll
             for (int j = 0; j < V; ++j) v[i][j] = 0.0f;
@@ -172,22 +213,28 @@ __global__ void __launch_bounds__(WARP ? 32 * WARP_ROWS : 512) q8_row_kernel(con
         }
     }
     if (MODE == Q8_NORM) {
-        Pack<float, V> pw[NV];
+        float w[NV][V];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (t + i * nt) * V;
-            if (c < p.C) pw[i].load(p.w + c);
+            const int c = column(i);
+            if constexpr (EDGE) {
+                if (whole(c) || some(c)) load_gains<V>(p.w, c, -phase & 3, p.C, w[i]);
+            } else {
+                if (whole(c)) {
+                    Pack<float, V> pw;
+                    pw.load(p.w + c);
+                    pw.unpack(w[i]);
+                }
+            }
         }
         const float r = row_rstd(row_sum<WARP>(ss, red), p.C, p.eps);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (t + i * nt) * V;
-            if (c < p.C) {
-                float w[V];
-                pw[i].unpack(w);
+            const int c = column(i);
+            if (whole(c) || some(c)) {
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    v[i][j] = v[i][j] * r * w[j];
+                    v[i][j] = v[i][j] * r * w[i][j];
                     top = max(top, abs_bits(v[i][j]));
                 }
             }
@@ -196,15 +243,20 @@ __global__ void __launch_bounds__(WARP ? 32 * WARP_ROWS : 512) q8_row_kernel(con
     float inv;
     const float s = row_scale(row_max<WARP>(top, redu), inv);
     if (t == 0) p.scale[row] = s;
-    int8_t* q = p.q + (size_t)row * p.ldq;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int c = (t + i * nt) * V;
-        if (c < p.C) {
+        const int c = column(i);
+        if (whole(c) || some(c)) {
             if (inv == 0.0f)
 #pragma unroll
                 for (int j = 0; j < V; ++j) v[i][j] = 0.0f;
-            store_codes<V>(q + c, v[i], inv);
+            if (whole(c)) {
+                store_codes<V>(q + c, v[i], inv);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (c + j >= 0 && c + j < p.C) q[c + j] = (int8_t)code_bits(v[i][j], inv);
+            }
         }
     }
 }
@@ -267,19 +319,19 @@ template <typename K> int launch(K kernel, unsigned grid, unsigned block, size_t
     return -9;
 }
 
-template <int MODE, typename TX, typename TY, int V, int NV> int launch_rows(const RowArgs& p, int threads, cudaStream_t st) {
+template <int MODE, typename TX, typename TY, int V, int NV, bool EDGE> int launch_rows(const RowArgs& p, int threads, cudaStream_t st) {
     if (threads == 32)
-        return launch(q8_row_kernel<MODE, TX, TY, V, NV, true>, (unsigned)((p.rows + WARP_ROWS - 1) / WARP_ROWS), 32 * WARP_ROWS, 0, p, st);
-    return launch(q8_row_kernel<MODE, TX, TY, V, NV, false>, (unsigned)p.rows, (unsigned)threads, 0, p, st);
+        return launch(q8_row_kernel<MODE, TX, TY, V, NV, true, EDGE>, (unsigned)((p.rows + WARP_ROWS - 1) / WARP_ROWS), 32 * WARP_ROWS, 0, p, st);
+    return launch(q8_row_kernel<MODE, TX, TY, V, NV, false, EDGE>, (unsigned)p.rows, (unsigned)threads, 0, p, st);
 }
 
 // Threads per row. Many rows: 32 or 16 values a thread, whichever leaves fewer of the row's threads idle (loads in flight are what counts:
 // 32768 x 960 fp32 with a warp per row 23.5 us, with 16 or 8 values a thread 34); SwiGLU, which loads two vectors for each value, two accesses
 // (32768 x 2560 bf16 60 to 65 us, four accesses 64 to 68, one 79); bf16 rows of 1024 to 2048 columns 64 values, a warp per row (16384 x 1536
 // 13.7 us against 17.7). Few rows: as many threads as there are vectors, so that a row costs one load's latency and two reductions.
-template <int MODE, typename TX, typename TY, int V> int launch_vec(const RowArgs& p, cudaStream_t st) {
-    const int vecs = (p.C + V - 1) / V;
-    constexpr bool LONG = MODE == Q8_ROWS && V == 8;
+template <int MODE, typename TX, typename TY, int V, bool EDGE> int launch_vec(const RowArgs& p, cudaStream_t st) {
+    const int vecs = EDGE ? (p.C + 2 * V - 2) / V : (p.C + V - 1) / V;   // a row that starts inside a vector may touch one more
+    constexpr bool LONG = MODE == Q8_ROWS && V == 8 && !EDGE;
     constexpr int MOST = V == 1 ? 16 : LONG ? 8 : 32 / V;   // accesses per thread (single elements: 16, or a block could not have 512 threads)
     const auto threads_for = [&](int n) { return ((vecs + n - 1) / n + 31) / 32 * 32; };
     const bool one_warp = LONG && vecs > 128 && vecs <= 256;
@@ -290,14 +342,14 @@ template <int MODE, typename TX, typename TY, int V> int launch_vec(const RowArg
     while (nv > 1 && threads_for(nv / 2) <= 512 && (long)p.rows * threads_for(nv) < 148L * 512) nv /= 2;
     const int threads = threads_for(nv);
     if constexpr (MOST >= 16) {
-        if (nv > 8) return launch_rows<MODE, TX, TY, V, 16>(p, threads, st);
+        if (nv > 8) return launch_rows<MODE, TX, TY, V, 16, EDGE>(p, threads, st);
     }
     if constexpr (MOST >= 8) {
-        if (nv > 4) return launch_rows<MODE, TX, TY, V, 8>(p, threads, st);
+        if (nv > 4) return launch_rows<MODE, TX, TY, V, 8, EDGE>(p, threads, st);
     }
-    if (nv > 2) return launch_rows<MODE, TX, TY, V, 4>(p, threads, st);
-    if (nv > 1) return launch_rows<MODE, TX, TY, V, 2>(p, threads, st);
-    return launch_rows<MODE, TX, TY, V, 1>(p, threads, st);
+    if (nv > 2) return launch_rows<MODE, TX, TY, V, 4, EDGE>(p, threads, st);
+    if (nv > 1) return launch_rows<MODE, TX, TY, V, 2, EDGE>(p, threads, st);
+    return launch_rows<MODE, TX, TY, V, 1, EDGE>(p, threads, st);
 }
 
 template <int MODE, typename TX, typename TY> int run_rows(const RowArgs& p, cudaStream_t st) {
@@ -309,12 +361,16 @@ template <int MODE, typename TX, typename TY> int run_rows(const RowArgs& p, cud
             if (cudaFuncSetAttribute(q8_wide_row_kernel<MODE, TX, TY>, cudaFuncAttributeMaxDynamicSharedMemorySize, Q8_MAX_COLUMNS * 4) != cudaSuccess) return -5;
         return launch(q8_wide_row_kernel<MODE, TX, TY>, (unsigned)p.rows, 1024, (size_t)p.C * 4, p, st);
     };
-    // Vectors of 16 bytes of x, and as many elements of everything else, where every row of every operand starts on such a boundary.
-    const auto fits = [](const void* ptr, int ld, size_t elem) { return ((uintptr_t)ptr % (V * elem > 16 ? 16 : V * elem)) == 0 && (ld % V) == 0; };
-    const bool vec = (p.C % V) == 0 && fits(p.x, p.ldx, sizeof(TX)) && fits(p.q, p.ldq, 1) && (!p.y || fits(p.y, p.ldy, sizeof(TY))) &&
-                     (!p.sum || fits(p.sum, p.lds, sizeof(TX))) && (!p.w || fits(p.w, V, sizeof(float)));
-    if (p.C > (vec ? VEC_MOST : SCALAR_MOST)) return wide();
-    return vec ? launch_vec<MODE, TX, TY, V>(p, st) : launch_vec<MODE, TX, TY, 1>(p, st);
+    // Vectors of 16 bytes of x, and as many elements of everything else, where every row of every operand starts on such a boundary, or on the
+    // same element behind one (contiguous tensors of an odd width). Others go element by element.
+    const auto begins = [](const void* ptr, size_t elem) { return (int)((uintptr_t)ptr / elem % V); };
+    const int at = begins(p.x, sizeof(TX)), step = p.ldx % V;
+    const bool same = begins(p.q, 1) == at && p.ldq % V == step && (!p.y || (begins(p.y, sizeof(TY)) == at && p.ldy % V == step)) &&
+                      (!p.sum || (begins(p.sum, sizeof(TX)) == at && p.lds % V == step)) && (!p.w || (uintptr_t)p.w % 16 == 0);
+    const bool vec = same && at == 0 && step == 0 && p.C % V == 0;
+    if (p.C > (vec ? VEC_MOST : same ? VEC_MOST - 2 * V : SCALAR_MOST)) return wide();
+    if (vec) return launch_vec<MODE, TX, TY, V, false>(p, st);
+    return same && p.C >= 8 * V ? launch_vec<MODE, TX, TY, V, true>(p, st) : launch_vec<MODE, TX, TY, 1, false>(p, st);
 }
 
 }  // namespace

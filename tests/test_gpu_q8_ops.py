@@ -162,6 +162,39 @@ def test_swiglu(be, dtype, rows, cols):
     check_codes(be.get(dq, (rows, cols), np_dtype=np.int8), be.get(ds, (rows,)), g / (1 + np.exp(-g)) * u, (2 * np.abs(g) + 12) * U)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(6000, 1001), (5000, 1535), (2500, 4099), (1300, 9003), (4000, 2048), (3000, 1536)])
+def test_many_rows(be, dtype, rows, cols):
+    """Enough rows that a thread holds as many values as it may; odd widths, whose rows start anywhere inside a vector. The unused operands of one
+    operator are those of another: rows as x, norm with an addend of either type, SwiGLU of two matrices."""
+    rng = rng_of(rows, cols, dtype, 21)
+    x, a = values(rng, rows, cols, dtype), values(rng, rows, cols, dtype, 0.5)
+    w = (1 + 0.2 * rng.standard_normal(cols)).astype(np.float32)
+    dx, da, dw = be.put(x, dtype), be.put(a, dtype), be.put(w)
+    dq, ds, dsum = filled(be, rows * cols + 64, 0x55), be.alloc(rows * 4), filled(be, rows * cols * 4 + 64, 0xFF)
+    e = 2 if dtype == BMC_BF16 else 4
+
+    def codes():
+        q = be.get(dq, (rows * cols + 64,), np_dtype=np.int8)
+        assert np.all(q[rows * cols:] == 0x55)
+        return q[:rows * cols].reshape(rows, cols), be.get(ds, (rows,))
+
+    assert be.lib.bmc_quantize_rows_q8(be.ctx, dtype, dq, cols, ds, dx, cols, rows, cols) == 0
+    check_codes(*codes(), x.astype(np.float64), 0.0)
+    assert be.lib.bmc_rmsnorm_q8(be.ctx, dtype, dq, cols, ds, dsum, cols, dx, cols, dtype, da, cols, dw, rows, cols, 1e-5) == 0
+    s, v = norm_ref(x, a, w, 1e-5)
+    check_codes(*codes(), v, (cols / 64 + 20) * U)
+    raw = be.get(dsum, (rows * cols * e + 64,), np_dtype=np.uint8)
+    assert np.all(raw[rows * cols * e:] == 0xFF)
+    assert np.all(np.abs(be.get(dsum, (rows, cols), dtype) - s) <= (U if dtype == BMC_F32 else U + 2.0 ** -8) * np.abs(s))
+    assert be.lib.bmc_swiglu_q8(be.ctx, dtype, dq, cols, ds, da, dx, cols, rows, cols) == 0
+    g, u = a.astype(np.float64), x.astype(np.float64)
+    check_codes(*codes(), g / (1 + np.exp(-g)) * u, (2 * np.abs(g) + 12) * U)
+    other = values(rng, rows, cols, BMC_F32 + BMC_BF16 - dtype, 0.5)
+    assert be.lib.bmc_rmsnorm_q8(be.ctx, dtype, dq, cols, ds, dx, cols, dx, cols, BMC_F32 + BMC_BF16 - dtype, be.put(other, BMC_F32 + BMC_BF16 - dtype), cols, dw, rows, cols, 1e-5) == 0
+    check_codes(*codes(), norm_ref(x, other, w, 1e-5)[1], (cols / 64 + 20) * U)
+
+
 @pytest.mark.parametrize("cols", [40, 961, 5000, 50000])
 def test_rows_that_cannot_be_scaled(be, cols):
     """Zeros, subnormal scales, the largest finite values, infinities and NaN, one kind a row."""
