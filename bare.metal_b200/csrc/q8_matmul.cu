@@ -4,14 +4,17 @@
 // product of the scales, their product, the residual's addition and the store: the result does not depend on the order of the sum, and a
 // reduction split over several CTAs is as exact (and as reproducible) as one that is not.
 //
-// Both kernels compute the transposed tile: the weights are the A operand (128 output channels = the 128 lanes of tensor memory), the tokens
-// the B operand (16 to 256 of them = accumulator columns). A warp then holds 32 consecutive channels of one token in one register across
-// its lanes, so that a plain store of that register is a contiguous 128-byte (fp32) or 64-byte (bf16) piece of an output row whatever its
-// alignment, the channel's scale is a register of the lane and the token's a broadcast from shared memory. Few tokens cost a narrow
+// The tensor-core kernels compute the transposed tile: the weights are the A operand (128 output channels = the 128 lanes of tensor memory),
+// the tokens the B operand (16 to 256 of them = accumulator columns). A warp then holds 32 consecutive channels of one token in one register
+// across its lanes, so that a plain store of that register is a contiguous 128-byte (fp32) or 64-byte (bf16) piece of an output row whatever
+// its alignment, the channel's scale is a register of the lane and the token's a broadcast from shared memory. Few tokens cost a narrow
 // instruction instead of an empty tile.
+//   q8_few_kernel    one to four tokens, without tensor cores: a warp per channel. 1 x 960 -> 1600 1.55 us.
 //   q8_split_kernel  one tile of 128 channels per cluster; the CTAs of the cluster split K and exchange their partial sums through
-//                    distributed shared memory. For outputs of too few tiles to fill the GPU: decode, short prompts.
-//   q8_pair_kernel   persistent CTA pairs with tiles of 256 channels x up to 256 tokens, for everything larger.
+//                    distributed shared memory. For outputs of too few tiles to fill the GPU: decode, short prompts. 64 x 2560 -> 960 with a
+//                    residual 4.2 us: 0.8 until the first bytes are there, 1.2 for five k-blocks, 0.6 for the exchange, 0.3 for the stores.
+//   q8_pair_kernel   persistent CTA pairs with tiles of 256 channels x up to 256 tokens, for everything larger. 8192 x 8192 -> 8192 341 us
+//                    (3.22 POP/s, 0.97 of twice the measured bf16 rate), 32768 x 960 -> 5120 131 to 137 us.
 #include "q8_kernels.cuh"
 
 #include <cuda.h>

@@ -8,7 +8,10 @@
 // rounds to 127 at most.
 //
 // All three are bound by memory: every input is read once and every output written once, the row stays in registers between the reductions
-// (up to 32 values a thread), so the threads of a row follow from its width.
+// (up to 32 values a thread), so the threads of a row follow from its width. Against the measured copy rate: rows 32768 x 960 fp32 23.5 us
+// (1.02), norm of an fp32 stream and a bf16 addend 52.9 us (1.00), SwiGLU 32768 x 2560 bf16 65.1 us (0.98); bf16 rows of middling widths 0.7
+// to 0.85, where a row is too short for its block's phases. One block or warp per row, without a loop: blocks that stay and walk the rows
+// were slower (62.8, 82 us), with a ring of bulk copies in front of them as well (56.5, 72 us).
 #include "q8_kernels.cuh"
 
 #include <cstdlib>
