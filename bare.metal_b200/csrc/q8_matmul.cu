@@ -122,8 +122,9 @@ __device__ __forceinline__ void report_abort(const Q8Args& p, volatile int* abor
 // memory, barriers and tensor maps costs more than the whole product of one token (1 x 960 -> 1600: 3.8 us there); here a call is a round
 // or two of loads and one reduction.
 constexpr int FEW_WARPS = 8, FEW_TOKENS = 4;
+// (No __restrict__: what the kernel in front writes must not come through the read-only path.)
 template <typename TO, bool RES, int MT>
-__global__ void __launch_bounds__(32 * FEW_WARPS) q8_few_kernel(const Q8Args p, const int8_t* __restrict__ q, int ldq, const int8_t* __restrict__ w) {
+__global__ void __launch_bounds__(32 * FEW_WARPS) q8_few_kernel(const Q8Args p, const int8_t* q, int ldq, const int8_t* w) {
     const int lane = threadIdx.x & 31, n = (int)blockIdx.x * FEW_WARPS + (int)(threadIdx.x >> 5), chunks = p.K >> 4;
     const int8_t* wr = w + (size_t)min(n, p.N - 1) * p.K;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -336,7 +337,7 @@ constexpr int KPS = 2;                    // k-blocks per ring stage: one wait a
 constexpr int PAIR_STAGES = 3;
 constexpr int HELD_BLOCKS = 8;
 constexpr int HELD_BN = 224;              // widest token tile whose ring fits beside 128 KB of weights
-constexpr int EPI_WARPS = 8;              // two per lane quarter, taking 32-column chunks in turn
+constexpr int EPI_WARPS = 8;              // two per lane quarter, taking 32-token chunks in turn
 constexpr int PAIR_THREADS = 96 + 32 * EPI_WARPS;   // warps 0 and 1 copy, warp 2 issues the products
 // All that a CTA may ask for, whatever the ring needs: a CTA of the split kernel must not run beside one of this kernel. Both hold tensor
 // memory while they wait for other CTAs of theirs; on two SMs (two streams) each could hold what the other's peer is still waiting to allocate.

@@ -255,14 +255,16 @@ int bmc_graph_launch(bmc_ctx_t* ctx);
 /* ---- 8-bit rows and their product (activations in 8 bits; no counterpart in the reference, whose Q8 / Q4 keep fp32 activations) ----
  * A matrix in 8 bits is int8 codes [rows][ld] and one fp32 scale per row; it stands for code * scale. Activations have a scale per token,
  * weights ([OC][C], rows = output channels) a scale per channel: bmc_quantize_rows_q8 makes both.
- *   row v[C]:  scale = max|v| / 127, code = rint(v * (1 / scale)), ties to even; codes lie in [-127, 127].
+ *   row v[C]:  scale = max|v| / 127, code = the integer nearest to v * (1 / scale), ties to even (1 / scale is rounded, the product is not);
+ *   codes lie in [-127, 127].
  *   A row whose scale would be subnormal (max|v| < 1.5e-36, zeros) is stored as scale 0 and codes 0. A row with an infinity or a NaN, in v
  *   or on the way to it (a sum of squares that overflows), is stored as scale NaN and codes 0: its products are NaN.
  * dtype / add_dtype: BMC_F32 or BMC_BF16, arithmetic in fp32. Every leading dimension is in elements and at least the row's width; columns
  * behind C are neither read nor written. Rows of any width 1 <= C <= BMC_Q8_MAX_COLUMNS and any alignment of their type; 16-byte aligned
  * pointers and leading dimensions take the vectorised path. Zero rows: 0 is returned and nothing is enqueued. Outputs may not overlap
  * inputs, except where said. Return values: 0, -1 (an argument out of range or a null pointer), -2 (a leading dimension that is no
- * multiple of what the call asks for), -3 (a misaligned pointer). Nothing is enqueued by a refused call.
+ * multiple of what the call asks for), -3 (a misaligned pointer). Nothing is enqueued by a refused call. bmc_status() reports 3000 after a
+ * product whose bounded waits ran out.
  *   quantize_rows : v = x
  *   rmsnorm       : v = s * rsqrt(mean(s^2) + eps) * w with s = x + add (add may be NULL: s = x); the norm takes s before it is rounded.
  *                   d_sum (may be NULL) receives s in dtype; it may be d_x itself (lds == ldx), or d_add (same dtype, lds == lda).
