@@ -8,6 +8,18 @@ namespace bmb {
 // widest row of the row kernels: one fp32 value per column in shared memory
 constexpr int Q8_MAX_COLUMNS = 57344;
 
+// Runs `setup` (0 = done, or a negative code) until it has succeeded once with the current device. The device is marked behind the set-up:
+// of two threads whose first calls meet, none launches a kernel whose attributes the other is still setting (setting them twice is harmless).
+template <typename Setup> int set_up_once(std::atomic<unsigned long long>& done_mask, const Setup& setup) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (done_mask.load(std::memory_order_acquire) & bit) return 0;
+    const int rc = setup();
+    if (rc == 0) done_mask.fetch_or(bit, std::memory_order_release);
+    return rc;
+}
+
 int q8_quantize_rows(int dtype, int8_t* q, int ldq, float* scale, const void* x, int ldx, int rows, int C, cudaStream_t st);
 // add, sum and their combination are optional (null); sum may be x or add
 int q8_rmsnorm(int dtype, int8_t* q, int ldq, float* scale, void* sum, int lds, const void* x, int ldx, int add_dtype, const void* add, int lda,

@@ -671,11 +671,12 @@ Plan choose(int M, int N, int K, int sms) {
 
 template <typename TO, bool RES> int launch(Q8Args p, const int8_t* q, int ldq, const int8_t* w, cudaStream_t st) {
     static std::atomic<unsigned long long> done{0};
-    if (first_use_on_current_device(done)) {
-        if (cudaFuncSetAttribute(q8_pair_kernel<TO, RES, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM) != cudaSuccess) return -5;
-        if (cudaFuncSetAttribute(q8_pair_kernel<TO, RES, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM) != cudaSuccess) return -5;
-        if (cudaFuncSetAttribute(q8_split_kernel<TO, RES>, cudaFuncAttributeMaxDynamicSharedMemorySize, split_smem(128, 2, MAX_STAGES)) != cudaSuccess) return -5;
-    }
+    const int rc = set_up_once(done, [] {
+        const auto allow = [](auto* kernel, int bytes) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess; };
+        return allow(q8_pair_kernel<TO, RES, false>, PAIR_SMEM) && allow(q8_pair_kernel<TO, RES, true>, PAIR_SMEM) &&
+               allow(q8_split_kernel<TO, RES>, split_smem(128, 2, MAX_STAGES)) ? 0 : -5;
+    });
+    if (rc) return rc;
     const int sms = sm_count_current_device();
     const Plan plan = choose(p.M, p.N, p.K, sms);
     static const bool overlap = getenv("BM_NO_PDL") == nullptr;

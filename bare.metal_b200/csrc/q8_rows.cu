@@ -360,8 +360,10 @@ template <int MODE, typename TX, typename TY> int run_rows(const RowArgs& p, cud
     constexpr int SCALAR_MOST = 16 * 512, VEC_MOST = 32 * 512;
     const auto wide = [&]() {
         static std::atomic<unsigned long long> done{0};
-        if (first_use_on_current_device(done))
-            if (cudaFuncSetAttribute(q8_wide_row_kernel<MODE, TX, TY>, cudaFuncAttributeMaxDynamicSharedMemorySize, Q8_MAX_COLUMNS * 4) != cudaSuccess) return -5;
+        const int rc = set_up_once(done, [] {
+            return cudaFuncSetAttribute(q8_wide_row_kernel<MODE, TX, TY>, cudaFuncAttributeMaxDynamicSharedMemorySize, Q8_MAX_COLUMNS * 4) == cudaSuccess ? 0 : -5;
+        });
+        if (rc) return rc;
         return launch(q8_wide_row_kernel<MODE, TX, TY>, (unsigned)p.rows, 1024, (size_t)p.C * 4, p, st);
     };
     // Vectors of 16 bytes of x, and as many elements of everything else, where every row of every operand starts on such a boundary, or on the

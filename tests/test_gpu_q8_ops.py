@@ -512,3 +512,51 @@ def test_first_use_in_a_capture():
     """A process whose first call of every kernel is being captured."""
     r = subprocess.run([sys.executable, "-c", FIRST_USE_IN_A_CAPTURE], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+FIRST_USE_BY_THREADS = """
+import sys, threading
+import numpy as np
+sys.path.insert(0, "bare.metal_b200"); sys.path.insert(0, "tests")
+import bmapi, bmcapi, test_gpu_q8_ops as t
+lib = bmapi.load_product()
+backends = [bmcapi.Backend(lib) for _ in range(4)]
+rng = np.random.default_rng(2)
+shapes = ((24, 2560, 130), (600, 960, 1600), (5000, 2048, 1600), (3, 960, 200))
+q = {K: rng.integers(-128, 128, (5000, K)).astype(np.int8) for K in (960, 2048, 2560)}
+w = {K: rng.integers(-128, 128, (1600, K)).astype(np.int8) for K in q}
+x = rng.standard_normal((3, 20000)).astype(np.float32)
+got, failed, gate = {}, [], threading.Barrier(4)
+def work(i):
+    try:
+        be = backends[i]
+        dq, dw = {K: t.put_bytes(be, q[K]) for K in q}, {K: t.put_bytes(be, w[K]) for K in w}
+        ds, dn = be.put(np.full(5000, 0.5, np.float32)), be.put(np.full(1600, 0.25, np.float32))
+        outs = [be.alloc(M * N * 4) for M, K, N in shapes]
+        dx, cq, cs = be.put(x), be.alloc(x.size), be.alloc(12)
+        gate.wait()
+        for _ in range(8):
+            for (M, K, N), out in zip(shapes, outs):
+                assert lib.bmc_matmul_q8(be.ctx, 0, out, N, dq[K], K, ds, dw[K], dn, None, 0, M, K, N) == 0
+            assert lib.bmc_quantize_rows_q8(be.ctx, 0, cq, 20000, cs, dx, 20000, 3, 20000) == 0
+        assert lib.bmc_sync(be.ctx) == 0
+        got[i] = [be.get(out, (M, N)) for (M, K, N), out in zip(shapes, outs)] + [be.get(cq, x.shape, np_dtype=np.int8), be.get(cs, (3,))]
+    except BaseException as e:
+        failed.append(e)
+        gate.abort()
+threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+[th.start() for th in threads]
+[th.join() for th in threads]
+assert not failed, failed
+for r in got.values():
+    for (M, K, N), out in zip(shapes, r):
+        want = (q[K][:M].astype(np.float64) @ w[K][:N].astype(np.float64).T) * 0.125
+        assert np.all(np.abs(out - want) <= 2.0 ** -24 * np.abs(want)), (M, K, N)
+    t.check_codes(r[4], r[5], x.astype(np.float64), 0.0)
+"""
+
+
+def test_first_use_by_threads_with_contexts_of_their_own():
+    """Four threads whose first calls meet, each on its own context's stream: every plan of the product beside the others."""
+    r = subprocess.run([sys.executable, "-c", FIRST_USE_BY_THREADS], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
