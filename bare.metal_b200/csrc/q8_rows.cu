@@ -324,7 +324,7 @@ template <typename K> int launch(K kernel, unsigned grid, unsigned block, size_t
 
 template <int MODE, typename TX, typename TY, int V, int NV, bool EDGE> int launch_rows(const RowArgs& p, int threads, cudaStream_t st) {
     if (threads == 32)
-        return launch(q8_row_kernel<MODE, TX, TY, V, NV, true, EDGE>, (unsigned)((p.rows + WARP_ROWS - 1) / WARP_ROWS), 32 * WARP_ROWS, 0, p, st);
+        return launch(q8_row_kernel<MODE, TX, TY, V, NV, true, EDGE>, ((unsigned)p.rows + WARP_ROWS - 1) / WARP_ROWS, 32 * WARP_ROWS, 0, p, st);
     return launch(q8_row_kernel<MODE, TX, TY, V, NV, false, EDGE>, (unsigned)p.rows, (unsigned)threads, 0, p, st);
 }
 

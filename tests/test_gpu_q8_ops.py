@@ -357,6 +357,22 @@ def test_offsets_beyond_32_bits(be):
     assert np.all(np.abs(out - ref) <= 3.01 * U * np.abs(ref))
 
 
+def test_the_largest_number_of_rows(be):
+    """2^31 - 1 rows of one column: every row is its own largest value."""
+    rows = 2 ** 31 - 1
+    dx, dq, ds = filled(be, rows * 4, 0x3F), filled(be, rows + 1, 0x55), filled(be, rows * 4, 0xFF)
+    last = np.array([-2.0, 0.0, 1e30], np.float32)
+    assert be.lib.bmc_upload(be.ctx, dx + (rows - 3) * 4, last.ctypes.data, 12) == 0
+    assert be.lib.bmc_quantize_rows_q8(be.ctx, BMC_F32, dq, 1, ds, dx, 1, rows, 1) == 0
+    assert be.lib.bmc_sync(be.ctx) == 0
+    assert list(be.get(dq + rows - 4, (5,), np_dtype=np.int8)) == [127, -127, 0, 127, 0x55]
+    value = np.frombuffer(b"\x3f" * 4, np.float32).astype(np.float64)[0]
+    ref = np.array([value, 2.0, 0.0, 1e30]) / 127.0
+    assert np.all(np.abs(be.get(ds + (rows - 4) * 4, (4,)) - ref) <= 2 * U * ref)
+    for first in (0, 2 ** 30 - 2, 2 ** 30 + 12345):
+        assert np.all(be.get(dq + first, (4,), np_dtype=np.int8) == 127)
+        assert np.all(np.abs(be.get(ds + first * 4, (4,)) - value / 127.0) <= 2 * U * value / 127.0)
+
 # ---- together --------------------------------------------------------------------------------------------------------------------------
 def mlp_inputs(rows, D, H, key=1):
     rng = rng_of(rows, D, H, key)
