@@ -15,6 +15,7 @@
 #include "q8_kernels.cuh"
 
 #include <cstdlib>
+#include <type_traits>
 
 namespace bmb {
 
@@ -126,32 +127,45 @@ template <bool WARP> __device__ __forceinline__ uint32_t row_max(uint32_t v, uin
 
 constexpr int WARP_ROWS = 4;   // rows per block where a warp has a row
 
-// V values from p[c ..] of a row that has `C` of them, those outside as 0
-template <typename T, int V> __device__ __forceinline__ void load_edge(const T* p, int c, int C, float (&f)[V]) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = c + j >= 0 && c + j < C ? to_f32(p[c + j]) : 0.0f;
-}
-// V gains from w[c ..], c = `off` (0 to 3) above a multiple of four: whole vectors, and a shift that is the same for every thread of a row
-template <int V> __device__ __forceinline__ void load_gains(const float* w, int c, int off, int C, float (&f)[V]) {
+// V gains from w[c ..], c = `off` (0 to 3) above a multiple of four: whole vectors, and a shift that is the same for every thread of a row.
+// Nothing in the branch uses a loaded value, so that all of a thread's loads are in flight together.
+template <int V> struct ShiftedGains {
     float t[V + 4];
-    if (c < 0 || c - off + V + 4 > C) {
-        load_edge<float, V>(w, c, C, f);
-        return;
+    __device__ __forceinline__ void load(const float* w, int c, int off, int C) {
+        const int b = c - off;
+#pragma unroll
+        for (int k = 0; k < V / 4; ++k) vector(w + b + 4 * k, 4 * k);
+        if (b + V + 4 <= C) {
+            vector(w + b + V, V);
+        } else {
+#pragma unroll
+            for (int j = V; j < V + 3; ++j) t[j] = b + j < C ? w[b + j] : 0.0f;
+        }
     }
-#pragma unroll
-    for (int k = 0; k < V / 4 + 1; ++k) {
-        const float4 x = *(const float4*)(w + c - off + 4 * k);
-        t[4 * k] = x.x; t[4 * k + 1] = x.y; t[4 * k + 2] = x.z; t[4 * k + 3] = x.w;
+    __device__ __forceinline__ void vector(const float* p, int at) {
+        const float4 x = *(const float4*)p;
+        t[at] = x.x; t[at + 1] = x.y; t[at + 2] = x.z; t[at + 3] = x.w;
     }
+    __device__ __forceinline__ void get(float (&f)[V], int off) const {
+        float u[V + 2];
 #pragma unroll
-    for (int j = 0; j < V + 2; ++j) t[j] = (off & 1) ? t[j + 1] : t[j];
+        for (int j = 0; j < V + 2; ++j) u[j] = (off & 1) ? t[j + 1] : t[j];
 #pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = (off & 2) ? t[j + 2] : t[j];
-}
+        for (int j = 0; j < V; ++j) f[j] = (off & 2) ? u[j + 2] : u[j];
+    }
+};
+// and where rows start on a vector
+template <int V> struct Gains {
+    Pack<float, V> v;
+    __device__ __forceinline__ void load(const float* w, int c, int, int) { v.load(w + c); }
+    __device__ __forceinline__ void get(float (&f)[V], int) const { v.unpack(f); }
+};
 
 // V elements per access, NV accesses per thread. WARP: a warp per row, WARP_ROWS rows per block; otherwise a block per row.
 // EDGE: rows that do not start on a vector (an odd width), but on the same element of one in every operand: the vectors lie where memory has
-// them, the first one `phase` elements before the row, and the first and last of a row are read and written element by element.
+// them, and the up to V - 1 elements in front of the first and behind the last are one element each of the first threads. (Their loads go out
+// with the others. Vectors that hang over a row's ends, element by element in one lane, were slower: norm of 8192 x 4099
+// bf16 + bf16 70.5 us against 52.7, rows 24.3 against 17.0.)
 template <int MODE, typename TX, typename TY, int V, int NV, bool WARP, bool EDGE>
 __global__ void __launch_bounds__(WARP ? 32 * WARP_ROWS : 512) q8_row_kernel(const RowArgs p) {
     __shared__ float red[32];
@@ -166,45 +180,37 @@ __global__ void __launch_bounds__(WARP ? 32 * WARP_ROWS : 512) q8_row_kernel(con
     TX* sum = MODE == Q8_NORM && p.sum ? (TX*)p.sum + (size_t)row * p.lds : nullptr;
     int8_t* q = p.q + (size_t)row * p.ldq;
     const bool has_y = MODE == Q8_SWIGLU || (MODE == Q8_NORM && p.y != nullptr);
-    const int phase = EDGE ? (int)(((uintptr_t)x / sizeof(TX)) & (V - 1)) : 0;
-    const auto column = [&](int i) { return (t + i * nt) * V - phase; };
-    const auto whole = [&](int c) { return EDGE ? c >= 0 && c + V <= p.C : c < p.C; };
-    const auto some = [&](int c) { return EDGE && c < p.C && c + V > 0; };   // of a vector that is not whole
+    const int front = EDGE ? (int)(-(uintptr_t)((uintptr_t)x / sizeof(TX)) & (V - 1)) : 0, back = EDGE ? (p.C - front) & (V - 1) : 0, end = p.C - back;
+    const auto column = [&](int i) { return front + (t + i * nt) * V; };
+    const bool single = EDGE && t < front + back;   // of 2 V - 2 at the most: a row has 32 threads or more
+    const int cs = t < front ? t : end + t - front;
+    const auto value = [&](float a, float b) { return !has_y ? a : MODE == Q8_SWIGLU ? silu(a) * b : a + b; };
     Pack<TX, V> px[NV];
     Pack<TY, V> py[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = column(i);
-        if (whole(c)) {
+        if (c < end) {
             px[i].load(x + c);
             if (has_y) py[i].load(y + c);
         }
     }
-    float v[NV][V];
+    float v[NV][V], one = 0.0f;
+    if (single) one = value(to_f32(x[cs]), has_y ? to_f32(y[cs]) : 0.0f);
     float ss = 0.0f;
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = column(i);
-        if (whole(c) || some(c)) {
-            if (whole(c)) px[i].unpack(v[i]);
-            else load_edge<TX, V>(x, c, p.C, v[i]);
+        if (c < end) {
+            px[i].unpack(v[i]);
             if (has_y) {
                 float f[V];
-                if (whole(c)) py[i].unpack(f);
-                else load_edge<TY, V>(y, c, p.C, f);
+                py[i].unpack(f);
 #pragma unroll
-                for (int j = 0; j < V; ++j) v[i][j] = MODE == Q8_SWIGLU ? silu(v[i][j]) * f[j] : v[i][j] + f[j];
+                for (int j = 0; j < V; ++j) v[i][j] = value(v[i][j], f[j]);
             }
-            if (sum) {
-                if (whole(c)) {
-                    Pack<TX, V>::store(sum + c, v[i]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < V; ++j)
-                        if (c + j >= 0 && c + j < p.C) sum[c + j] = from_f32<TX>(v[i][j]);
-                }
-            }
+            if (sum) Pack<TX, V>::store(sum + c, v[i]);
         } else {
 #pragma unroll
             for (int j = 0; j < V; ++j) v[i][j] = 0.0f;
@@ -215,32 +221,33 @@ __global__ void __launch_bounds__(WARP ? 32 * WARP_ROWS : 512) q8_row_kernel(con
             else top = max(top, abs_bits(v[i][j]));
         }
     }
+    if (EDGE) {
+        if (single && sum) sum[cs] = from_f32<TX>(one);
+        if (MODE == Q8_NORM) ss = fmaf(one, one, ss);
+        else top = max(top, abs_bits(one));
+    }
     if (MODE == Q8_NORM) {
-        float w[NV][V];
+        std::conditional_t<EDGE, ShiftedGains<V>, Gains<V>> w[NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = column(i);
-            if constexpr (EDGE) {
-                if (whole(c) || some(c)) load_gains<V>(p.w, c, -phase & 3, p.C, w[i]);
-            } else {
-                if (whole(c)) {
-                    Pack<float, V> pw;
-                    pw.load(p.w + c);
-                    pw.unpack(w[i]);
-                }
-            }
-        }
+        for (int i = 0; i < NV; ++i)
+            if (column(i) < end) w[i].load(p.w, column(i), front & 3, p.C);
+        const float w1 = single ? p.w[cs] : 0.0f;
         const float r = row_rstd(row_sum<WARP>(ss, red), p.C, p.eps);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = column(i);
-            if (whole(c) || some(c)) {
+            if (column(i) < end) {
+                float g[V];
+                w[i].get(g, front & 3);
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    v[i][j] = v[i][j] * r * w[i][j];
+                    v[i][j] = v[i][j] * r * g[j];
                     top = max(top, abs_bits(v[i][j]));
                 }
             }
+        }
+        if (single) {
+            one = one * r * w1;
+            top = max(top, abs_bits(one));
         }
     }
     float inv;
@@ -249,19 +256,14 @@ __global__ void __launch_bounds__(WARP ? 32 * WARP_ROWS : 512) q8_row_kernel(con
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = column(i);
-        if (whole(c) || some(c)) {
+        if (c < end) {
             if (inv == 0.0f)
 #pragma unroll
                 for (int j = 0; j < V; ++j) v[i][j] = 0.0f;
-            if (whole(c)) {
-                store_codes<V>(q + c, v[i], inv);
-            } else {
-#pragma unroll
-                for (int j = 0; j < V; ++j)
-                    if (c + j >= 0 && c + j < p.C) q[c + j] = (int8_t)code_bits(v[i][j], inv);
-            }
+            store_codes<V>(q + c, v[i], inv);
         }
     }
+    if (single) q[cs] = inv == 0.0f ? 0 : (int8_t)code_bits(one, inv);
 }
 
 // Rows that 512 threads cannot hold in registers: a block per row, the row in shared memory between the passes.
@@ -333,13 +335,14 @@ template <int MODE, typename TX, typename TY, int V, int NV, bool EDGE> int laun
 // (32768 x 2560 bf16 60 to 65 us, four accesses 64 to 68, one 79); bf16 rows of 1024 to 2048 columns 64 values, a warp per row (16384 x 1536
 // 13.7 us against 17.7). Few rows: as many threads as there are vectors, so that a row costs one load's latency and two reductions.
 template <int MODE, typename TX, typename TY, int V, bool EDGE> int launch_vec(const RowArgs& p, cudaStream_t st) {
-    const int vecs = EDGE ? (p.C + 2 * V - 2) / V : (p.C + V - 1) / V;   // a row that starts inside a vector may touch one more
+    const int vecs = EDGE ? p.C / V : (p.C + V - 1) / V;
     constexpr bool LONG = MODE == Q8_ROWS && V == 8 && !EDGE;
     constexpr int MOST = V == 1 ? 16 : LONG ? 8 : 32 / V;   // accesses per thread (single elements: 16, or a block could not have 512 threads)
     const auto threads_for = [&](int n) { return ((vecs + n - 1) / n + 31) / 32 * 32; };
     const bool one_warp = LONG && vecs > 128 && vecs <= 256;
     int nv = LONG && !one_warp ? MOST / 2 : MOST;
     if (MODE == Q8_SWIGLU && V > 1) nv = 2;
+    if (MODE == Q8_NORM && EDGE) nv = MOST / 2;   // shifted gains hold up to twice the registers: 8192 x 4099 fp32 + bf16 61.9 us against 68.6
     while (threads_for(nv) > 512) nv *= 2;
     if (!one_warp && threads_for(nv / 2) <= 512 && threads_for(nv / 2) * (nv / 2) < threads_for(nv) * nv) nv /= 2;
     while (nv > 1 && threads_for(nv / 2) <= 512 && (long)p.rows * threads_for(nv) < 148L * 512) nv /= 2;
@@ -373,7 +376,7 @@ template <int MODE, typename TX, typename TY> int run_rows(const RowArgs& p, cud
     const bool same = begins(p.q, 1) == at && p.ldq % V == step && (!p.y || (begins(p.y, sizeof(TY)) == at && p.ldy % V == step)) &&
                       (!p.sum || (begins(p.sum, sizeof(TX)) == at && p.lds % V == step)) && (!p.w || (uintptr_t)p.w % 16 == 0);
     const bool vec = same && at == 0 && step == 0 && p.C % V == 0;
-    if (p.C > (vec ? VEC_MOST : same ? VEC_MOST - 2 * V : SCALAR_MOST)) return wide();
+    if (p.C / V > VEC_MOST / V || (!same && p.C > SCALAR_MOST)) return wide();
     if (vec) return launch_vec<MODE, TX, TY, V, false>(p, st);
     return same && p.C >= 8 * V ? launch_vec<MODE, TX, TY, V, true>(p, st) : launch_vec<MODE, TX, TY, 1, false>(p, st);
 }

@@ -128,6 +128,31 @@ def test_rmsnorm(be, dtype, add_dtype, rows, cols):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [33, 65, 71, 72, 1537, 4093, 16385, 16391])
+@pytest.mark.parametrize("shift", [0, 1, 6, 15])
+def test_rows_that_start_inside_a_vector(be, dtype, cols, shift):
+    """Contiguous rows from the same element on in every operand: each row starts at another element of a vector. Eight rows see them all."""
+    rows, rng = 8, rng_of(cols, shift, dtype, 5)
+    x, a, w = values(rng, rows, cols, dtype), values(rng, rows, cols, dtype, 0.5), (1 + 0.2 * rng.standard_normal(cols)).astype(np.float32)
+    dx, da, dw = put_rows(be, x, dtype, cols, shift), put_rows(be, a, dtype, cols, shift), be.put(w)
+    n, size = rows * cols, 2 if dtype == BMC_BF16 else 4
+    for norm in (True, False):
+        dq, ds, dsum = filled(be, n + 64, 0x55), filled(be, (rows + 1) * 4, 0x55), filled(be, (n + 64) * size, 0x55)
+        if norm:
+            assert be.lib.bmc_rmsnorm_q8(be.ctx, dtype, dq + shift, cols, ds, dsum + shift * size, cols, dx, cols, dtype, da, cols, dw, rows, cols, 1e-5) == 0
+            s, v = norm_ref(x, a, w, 1e-5)
+            raw = be.get(dsum, ((n + 64) * size,), np_dtype=np.uint8)
+            assert np.all(raw[:shift * size] == 0x55) and np.all(raw[(shift + n) * size:] == 0x55)
+            got = be.get(dsum + shift * size, (rows, cols), dtype)
+            assert np.all(np.abs(got - s) <= (U if dtype == BMC_F32 else U + 2.0 ** -8) * np.abs(s))
+        else:
+            assert be.lib.bmc_quantize_rows_q8(be.ctx, dtype, dq + shift, cols, ds, dx, cols, rows, cols) == 0
+            v = x.astype(np.float64)
+        q, sc = be.get(dq, (n + 64,), np_dtype=np.int8), be.get(ds, (rows + 1,))
+        assert np.all(q[:shift] == 0x55) and np.all(q[shift + n:] == 0x55) and sc[rows:].view(np.int32)[0] == 0x55555555
+        check_codes(q[shift:shift + n].reshape(rows, cols), sc[:rows], v, (cols / 64 + 20) * U if norm else 0.0)
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("cols", [33, 960, 4100, 40000])
 def test_rmsnorm_sum_in_place_and_left_out(be, dtype, cols):
     rows, rng = 9, rng_of(cols, dtype, 3)
